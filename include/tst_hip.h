@@ -554,6 +554,142 @@ typedef struct tst_select_step {
 int tst_select_step_run(const tst_select_step* s, const tst_rows* cur, const tst_rows* nxt, int64_t n_sent, int64_t k_in,
                         int64_t step, uint32_t sample_step, int last_step, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * Prompted decoding: a batch of prompts of DIFFERENT lengths is run through the model at once (packed, one row per token),
+ * its keys and values are kept in 4 bits in pages that a table maps per sequence, and decoding continues one token per row.
+ * The reference feeds a prefix by running the model on it (active_seqs, /root/reference/src/inference.py:37,132); it has no
+ * cache and every prefix of a batch has the same length.  These entry points came after version 109 and change nothing that
+ * existed; a host that binds at run time tests for the symbol.
+ * --------------------------------------------------------------------------------------------------------------------- */
+
+/* Page table and slot maps of B sequences from their lengths.  Sequence b needs ceil((lens[b] + room[b]) / page) pages (at most
+ * `width`; negative lengths count as 0; room NULL: 0): `room` is what decoding will add.  Pages are taken from pages[0..n_pages) in
+ * order, sequence after sequence: table[b][j] (ld = width) = the j-th page of sequence b, -1 beyond its need and where the list is
+ * exhausted.  cu [B + 1]: exclusive sums of lens.  For every token i of the packed batch (cu[b] <= i < cu[b + 1], i < N):
+ * pos[i] = i - cu[b], seq[i] = b, slots[i] = table[b][pos / page] * page + pos % page, or -1 where there is no page; entries at and
+ * behind cu[B] are left as they were.  used[0] = pages needed in all: more than n_pages means the list was too short.  page is a
+ * power of two in 8 .. 1024; the sum of lens must stay below 2^31, and n_pages * page too (slots are 32-bit; the cache's BYTES may
+ * pass 32 bits).  One launch. */
+int tst_page_plan(const int32_t* lens, const int32_t* room, int64_t B, const int32_t* pages, int64_t n_pages, int64_t page,
+                  int32_t* table, int64_t width, int32_t* cu, int32_t* slots, int32_t* pos, int32_t* seq, int64_t N, int32_t* used,
+                  void* stream);
+
+/* The same for one decode step: row r continues sequence s = sent[r] (sent NULL: s = r), whose token number base[s] + t it is:
+ * pos[r] = base[s] + t, lens[r] = pos[r] + 1 (what the row attends to), slots[r] = its slot, -1 without a page.  A row whose
+ * sequence is outside 0 .. n_seq - 1 gets pos 0, lens 0, slot -1. */
+int tst_page_step(const int32_t* base, const int32_t* sent, int64_t t, const int32_t* table, int64_t width, int64_t n_seq,
+                  int64_t page, int32_t* slots, int32_t* pos, int32_t* lens, int64_t R, void* stream);
+
+/* Causal attention over whole prompts, packed one behind the other: rows cu[b] .. cu[b + 1] - 1 are sequence b (cu [B + 1] int32 on
+ * the device, ascending, cu[B] <= N; sequences may be empty).  For row i of sequence b and head h, with g = h / (heads / kv_heads):
+ *     out[i][h] = sum_{j = cu[b]}^{i} w_j v[j][g],   w = softmax_j(scale * q[i][h] . k[j][g])
+ * q [N][ldq >= heads * dh], k, v [N][ld >= kv_heads * dh] (heads side by side in a row: views of a fused projection's output will
+ * do), out [N][ldo >= heads * dh], which must not overlap them.  Rows outside every sequence are left as they were.  What a row does
+ * not attend to never reaches it, NaN and infinities there included.
+ * Replaces the self-attention of a model run on whole prefixes (/root/reference/src/inference.py:132).
+ * heads % kv_heads == 0; dh <= 256, a multiple of 8 (bf16) or 4 (fp32); leading dimensions likewise, 16-byte aligned pointers.
+ * Scores, softmax and sums are fp32; the bf16 form rounds the weights to bf16 for the product with v, and the result once. */
+int tst_attn_prompt_f32(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv, const int32_t* cu,
+                        int64_t B, float* out, int64_t ldo, int64_t N, int64_t heads, int64_t kv_heads, int64_t dh, float scale,
+                        void* stream);
+int tst_attn_prompt_bf16(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const int32_t* cu,
+                         int64_t B, void* out, int64_t ldo, int64_t N, int64_t heads, int64_t kv_heads, int64_t dh, float scale,
+                         void* stream);
+
+/* A key / value cache in 4 bits (one layer; host struct of device pointers).  32 consecutive elements of a head share a power of
+ * two 2^E, E the smallest exponent in [-126, 126] with max|x| <= 6 * 2^E; an element is the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 to
+ * |x| * 2^-E (a tie goes to the even code) with its sign: 1 sign bit, 2 exponent bits, 1 mantissa bit.  The scale byte is E + 127.  A
+ * group that holds a NaN or an infinity gets scale byte 255 and stands for 32 NaN.  4.25 bits per element.
+ *   kc [pages][kv_heads][page][dh / 2]   key codes, elements 2 i (low half) and 2 i + 1 of a token in byte i
+ *   ks [pages][kv_heads][page][dh / 32]  their scale bytes
+ *   vc [pages][kv_heads][dh / 2][page]   value codes, same bytes, token by token along the last axis
+ *   vs [pages][kv_heads][dh / 32][page]
+ * dh is 32, 64, 128 or 256; page 16, 32, 64 or 128; all four arrays 16-byte aligned; slot = page number * page + token in page. */
+typedef struct tst_cache4 {
+    uint8_t *kc, *ks, *vc, *vs;
+    int64_t pages;
+    int32_t page, kv_heads, dh, reserved;
+} tst_cache4;
+
+/* Stores row i of k and v ([n][ld >= kv_heads * dh]) at slots[i]; a slot outside 0 .. pages * page - 1 stores nothing.  No slot may
+ * appear twice in one call (which row it would keep is not defined).  ld a multiple of 8 (bf16) / 4 (fp32), 16-byte aligned rows. */
+int tst_cache4_write_f32(const tst_cache4* c, const float* k, int64_t ldk, const float* v, int64_t ldv, const int32_t* slots,
+                         int64_t n, void* stream);
+int tst_cache4_write_bf16(const tst_cache4* c, const void* k, int64_t ldk, const void* v, int64_t ldv, const int32_t* slots,
+                          int64_t n, void* stream);
+/* Reads rows back as the values the codes stand for (exact in bf16 too, but for E + 2 > 127); a slot outside the cache gives zeros. */
+int tst_cache4_read_f32(const tst_cache4* c, const int32_t* slots, float* k, int64_t ldk, float* v, int64_t ldv, int64_t n,
+                        void* stream);
+int tst_cache4_read_bf16(const tst_cache4* c, const int32_t* slots, void* k, int64_t ldk, void* v, int64_t ldv, int64_t n,
+                         void* stream);
+
+/* One decode step's attention over that cache: row r attends to tokens 0 .. lens[r] - 1 of sequence s = seq[r] (seq NULL: s = r),
+ * token p in slot table[s][p / page] * page + p % page (table [n_seq][width]); lens is cut to max_len and to width * page.
+ *     out[r][h] = sum_p w_p V[p][g],   w = softmax_p(scale * q[r][h] . K[p][g]),   g = h / (heads / kv_heads)
+ * A row with nothing to attend to (length 0 or less, a sequence outside 0 .. n_seq - 1) gives zeros; a page number outside the cache
+ * counts as nothing to attend to.  q and out are fp32 or bf16 [R][ld >= heads * dh]; the keys and values enter the matrix cores as
+ * they are (every code is exact in bf16); scores, softmax and sums are fp32.  heads % kv_heads == 0.
+ * max_len: an upper bound of lens known to the host.  work: tst_attn_cache4_work floats of scratch (may be NULL when that is 0),
+ * written before it is read, not shared with a call that may run at the same time. */
+int64_t tst_attn_cache4_work(int64_t R, int64_t heads, int64_t kv_heads, int64_t dh, int64_t max_len);
+int tst_attn_cache4_f32(const tst_cache4* c, const float* q, int64_t ldq, const int32_t* table, int64_t width, int64_t n_seq,
+                        const int32_t* seq, const int32_t* lens, int64_t max_len, float* out, int64_t ldo, int64_t R, int64_t heads,
+                        float scale, float* work, int64_t n_work, void* stream);
+int tst_attn_cache4_bf16(const tst_cache4* c, const void* q, int64_t ldq, const int32_t* table, int64_t width, int64_t n_seq,
+                         const int32_t* seq, const int32_t* lens, int64_t max_len, void* out, int64_t ldo, int64_t R, int64_t heads,
+                         float scale, float* work, int64_t n_work, void* stream);
+
+/* Rules on the logits of a step, applied before the token selection (which has none in the reference,
+ * /root/reference/src/inference.py:132-149).  Every part may be absent (NULL).  For row r, s = sent[r] (sent NULL: r):
+ *   c = how often token v is among hist[r][0..hist_len[r]) (hist_len NULL: n_hist entries), p = v is among
+ *   prompt[prompt_cu[s] .. prompt_cu[s + 1]); ids outside 0 .. V - 1 are ignored
+ *   y = x[v]
+ *   if (c > 0 || p)  y = y > 0 ? y / params[s][0] : y * params[s][0]             repetition
+ *   if (c > 0)       y = (y - c * params[s][1]) - params[s][2]                   frequency, presence (generated tokens only)
+ *   y = y + bias[bias_row[r]][v]                                                 bias_row NULL: row 0; a row outside 0..n_bias-1: none
+ *   if bit v % 32 of mask[mask_row[r]][v / 32] is 0:  y = -inf                   mask_row likewise
+ * in fp32, in this order, rounded once where the logits are bf16.  params [n_sent][3] floats is required with hist or prompt. */
+typedef struct tst_logit_rules {
+    const float* params;
+    const int32_t* sent;         int64_t n_sent;   /* rows of params and entries of prompt_cu - 1; a row with s outside gets no penalty */
+    const int32_t* hist;         int64_t ld_hist;  int64_t n_hist;   /* hist_len entries are cut to n_hist */
+    const int32_t* hist_len;
+    const int32_t* prompt;       int64_t n_prompt;
+    const int32_t* prompt_cu;                      /* [n_sent + 1] */
+    const float* bias;           int64_t ld_bias;  int64_t n_bias;
+    const int32_t* bias_row;
+    const uint32_t* mask;        int64_t ld_mask;  int64_t n_masks;
+    const int32_t* mask_row;
+} tst_logit_rules;
+
+/* out[r][0..V) = the adjusted logits; out may be logits itself (same ld), else it must not overlap it. */
+int tst_adjust_logits_f32(const float* logits, int64_t ld, int64_t R, int64_t V, const tst_logit_rules* rules, float* out,
+                          int64_t ldo, void* stream);
+int tst_adjust_logits_bf16(const void* logits, int64_t ld, int64_t R, int64_t V, const tst_logit_rules* rules, void* out,
+                           int64_t ldo, void* stream);
+
+/* Grammar states after a step: out[r] = next[state[parent[r]]][tok[r]] for r < R (parent NULL: r; next [n_states][V]); -1, the state
+ * without a rule, stays -1, and so becomes whatever leaves the table (a parent outside 0 .. R_old - 1, a state or token outside it). */
+int tst_grammar_next(const int32_t* next, int64_t n_states, int64_t V, const int32_t* state, int64_t R_old, const int32_t* parent,
+                     const int32_t* tok, int32_t* out, int64_t R, void* stream);
+
+/* One decode step of a transformer decoder stack without cross-attention (tst_tfm_step_run's model) whose rows stand at positions of
+ * their own and whose self-attention reads a 4-bit paged cache: tst_page_step, embedding (pe[pos[r]]), per layer LayerNorm, q|k|v into
+ * qkv, tst_cache4_write, tst_attn_cache4, output projection + residual, feed-forward; final LayerNorm; vocabulary projection into
+ * step->logits.  `step` is the plan of tst_tfm_step_run (its caches, n_pos, anc_ld, part and argmax_keys are not used; n_pos bounds the
+ * positions).  Host structs. */
+typedef struct tst_paged_step {
+    const tst_tfm_step* step;
+    const tst_cache4* caches;    /* host array of step->n_layers */
+    const int32_t* table;        int64_t width;   int64_t n_seq;
+    const int32_t* base;         /* [n_seq] tokens of every sequence that the cache held before step 0 */
+    int32_t *slots, *pos, *lens; /* [rows] work */
+    void* qkv;                   /* [rows][3 d] work, the activation type */
+    float* work;                 int64_t n_work;  /* for tst_attn_cache4 */
+    int64_t max_len;             /* upper bound of base + t + 1 over all steps */
+} tst_paged_step;
+int tst_paged_step_run(const tst_paged_step* p, const int32_t* tok, const int32_t* sent, int64_t R, int64_t t, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -75,6 +75,26 @@ class TstSelectStep(ctypes.Structure):
                 ('am_keys', c_vp), ('n_alive_host', c_vp)]
 
 
+class TstCache4(ctypes.Structure):
+    """``tst_cache4`` of include/tst_hip.h"""
+    _fields_ = [('kc', c_vp), ('ks', c_vp), ('vc', c_vp), ('vs', c_vp), ('pages', c_i64), ('page', c_i32), ('kv_heads', c_i32), ('dh', c_i32),
+                ('reserved', c_i32)]
+
+
+class TstLogitRules(ctypes.Structure):
+    """``tst_logit_rules`` of include/tst_hip.h"""
+    _fields_ = [('params', c_vp), ('sent', c_vp), ('n_sent', c_i64), ('hist', c_vp), ('ld_hist', c_i64), ('n_hist', c_i64), ('hist_len', c_vp),
+                ('prompt', c_vp), ('n_prompt', c_i64), ('prompt_cu', c_vp), ('bias', c_vp), ('ld_bias', c_i64), ('n_bias', c_i64),
+                ('bias_row', c_vp), ('mask', c_vp), ('ld_mask', c_i64), ('n_masks', c_i64), ('mask_row', c_vp)]
+
+
+class TstPagedStep(ctypes.Structure):
+    """``tst_paged_step`` of include/tst_hip.h"""
+    _fields_ = [('step', ctypes.POINTER(TstTfmStep)), ('caches', ctypes.POINTER(TstCache4)), ('table', c_vp), ('width', c_i64), ('n_seq', c_i64),
+                ('base', c_vp), ('slots', c_vp), ('pos', c_vp), ('lens', c_vp), ('qkv', c_vp), ('work', c_vp), ('n_work', c_i64),
+                ('max_len', c_i64)]
+
+
 STEP_EMBED, STEP_LAYERS, STEP_VOCAB, STEP_FUSED_CELL = 1, 2, 4, 8
 
 _PROTOS = {
@@ -142,6 +162,21 @@ _PROTOS = {
                             c_i64, c_i64, c_i64, c_i32, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp], c_int),
     'tst_retire_compact_noalloc': ([ctypes.POINTER(TstRows), ctypes.POINTER(TstRows), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
                                     c_i64, c_i64, c_i64, c_i32, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp], c_int),
+    'tst_page_plan': ([c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp], c_int),
+    'tst_page_step': ([c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp], c_int),
+    'tst_attn_prompt_f32': ([c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_f32, c_vp], c_int),
+    'tst_attn_prompt_bf16': ([c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_f32, c_vp], c_int),
+    'tst_cache4_write_f32': ([ctypes.POINTER(TstCache4), c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp], c_int),
+    'tst_cache4_write_bf16': ([ctypes.POINTER(TstCache4), c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp], c_int),
+    'tst_cache4_read_f32': ([ctypes.POINTER(TstCache4), c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp], c_int),
+    'tst_cache4_read_bf16': ([ctypes.POINTER(TstCache4), c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp], c_int),
+    'tst_attn_cache4_work': ([c_i64, c_i64, c_i64, c_i64, c_i64], c_i64),
+    'tst_attn_cache4_f32': ([ctypes.POINTER(TstCache4), c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_f32, c_vp, c_i64, c_vp], c_int),
+    'tst_attn_cache4_bf16': ([ctypes.POINTER(TstCache4), c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_f32, c_vp, c_i64, c_vp], c_int),
+    'tst_adjust_logits_f32': ([c_vp, c_i64, c_i64, c_i64, ctypes.POINTER(TstLogitRules), c_vp, c_i64, c_vp], c_int),
+    'tst_adjust_logits_bf16': ([c_vp, c_i64, c_i64, c_i64, ctypes.POINTER(TstLogitRules), c_vp, c_i64, c_vp], c_int),
+    'tst_grammar_next': ([c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp], c_int),
+    'tst_paged_step_run': ([ctypes.POINTER(TstPagedStep), c_vp, c_vp, c_i64, c_i64, c_vp], c_int),
 }
 
 EXPORTS = tuple(_PROTOS)

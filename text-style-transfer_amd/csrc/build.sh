@@ -8,7 +8,7 @@ OUT=../libtst_hip.so
 # No packed fp32 instructions: some of their forms have given wrong results on this hardware now and then (the host pass does not
 # know the feature and says so: harmless).
 FLAGS="--offload-arch=gfx950 -O3 -fPIC -ffp-contract=off -std=c++17 -Wall -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
-UNITS="capi gemm_f32 gemm_f32_wreg gemm_f32_dma chain_f32 gemm_bf16 gru_fused rowops attn attn_mfma select gumbel step"
+UNITS="capi gemm_f32 gemm_f32_wreg gemm_f32_dma chain_f32 gemm_bf16 gru_fused rowops attn attn_mfma select gumbel paged cache4 prompt rules step"
 pids=()
 for f in $UNITS; do
   if [ ! -f $f.o ] || [ $f.hip -nt $f.o ] || [ build.sh -nt $f.o ] || [ tst_common.h -nt $f.o ] || [ ../../include/tst_hip.h -nt $f.o ]; then

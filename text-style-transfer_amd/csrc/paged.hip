@@ -1,0 +1,160 @@
+// Page tables and slot maps of a paged cache, built on the GPU from the lengths of the sequences (integers only).
+//
+// A launch is split over groups of adjacent sequences (blockIdx.x) and, within a group, over its tokens (blockIdx.y).  Every
+// workgroup first adds up the tokens and pages of ALL sequences in front of its group: at most a few thousand lengths out of
+// the L2, cheaper than a second launch that would wait for a scan (a launch costs about 2 us, the sum under 1 us at 1000
+// sequences and about 4 us at 8192).  Then it scans its own group in LDS and writes table rows and token entries, consecutive
+// lanes writing consecutive words.
+#include "tst_common.h"
+
+namespace {
+
+constexpr int MAX_GROUP = 64;   // sequences per workgroup: one lane each in the group's scan
+
+struct PlanArgs {
+    const int32_t *lens, *room, *pages;
+    int32_t *table, *cu, *slots, *pos, *seq, *used;
+    int64_t B, n_pages, N, width;
+    int page_shift, group;
+};
+
+__device__ __forceinline__ int64_t tokens_of(const PlanArgs& a, int64_t b) { return max(a.lens[b], 0); }
+__device__ __forceinline__ int64_t need_of(const PlanArgs& a, int64_t b, int64_t tokens) {
+    const int64_t room = a.room != nullptr ? max(a.room[b], 0) : 0;
+    const int64_t need = (tokens + room + (1 << a.page_shift) - 1) >> a.page_shift;
+    return need < a.width ? need : a.width;
+}
+__device__ __forceinline__ int32_t clip31(int64_t v) { return v > 0x7fffffff ? 0x7fffffff : (int32_t)v; }
+
+__global__ __launch_bounds__(256) void page_plan_kernel(PlanArgs a) {
+    __shared__ int64_t part[2][4];
+    __shared__ int64_t tok0[MAX_GROUP + 1], page0[MAX_GROUP + 1];
+    const int t = threadIdx.x, lane = t & 63;
+    const int64_t b0 = (int64_t)blockIdx.x * a.group;
+    const int nb = (int)min((int64_t)a.group, a.B - b0);
+    int64_t st = 0, sp = 0;
+    for (int64_t b = t; b < b0; b += 256) {
+        const int64_t n = tokens_of(a, b);
+        st += n;
+        sp += need_of(a, b, n);
+    }
+    for (int off = 32; off > 0; off >>= 1) {
+        st += __shfl_xor(st, off, 64);
+        sp += __shfl_xor(sp, off, 64);
+    }
+    if (lane == 0) { part[0][t >> 6] = st; part[1][t >> 6] = sp; }
+    __syncthreads();
+    if (t < 64) {   // scan of the group: one sequence per lane
+        int64_t n = 0, p = 0;
+        if (lane < nb) {
+            n = tokens_of(a, b0 + lane);
+            p = need_of(a, b0 + lane, n);
+        }
+        int64_t in = n, ip = p;
+        for (int off = 1; off < 64; off <<= 1) {
+            const int64_t un = __shfl_up(in, off, 64), up = __shfl_up(ip, off, 64);
+            if (lane >= off) { in += un; ip += up; }
+        }
+        const int64_t bt = part[0][0] + part[0][1] + part[0][2] + part[0][3], bp = part[1][0] + part[1][1] + part[1][2] + part[1][3];
+        tok0[lane] = bt + in - n;
+        page0[lane] = bp + ip - p;
+        if (lane == 63) { tok0[64] = bt + in; page0[64] = bp + ip; }
+    }
+    __syncthreads();
+    // entries of tok0 / page0 behind the group's last sequence hold the group's totals
+    const int64_t t_end = tok0[MAX_GROUP], p_end = page0[MAX_GROUP];
+    if (blockIdx.y == 0) {
+        if (t < nb) a.cu[b0 + t] = clip31(tok0[t]);
+        if (t == 0 && b0 + nb == a.B) {
+            a.cu[a.B] = clip31(t_end);
+            a.used[0] = clip31(p_end);
+        }
+    }
+    // table rows of the group, entry by entry
+    const int64_t cells = (int64_t)nb * a.width;
+    for (int64_t i = (int64_t)blockIdx.y * 256 + t; i < cells; i += (int64_t)gridDim.y * 256) {
+        const int s = (int)(i / a.width);
+        const int64_t j = i - (int64_t)s * a.width, at = page0[s] + j;
+        a.table[(b0 + s) * a.width + j] = (at < page0[s + 1] && at < a.n_pages) ? a.pages[at] : -1;
+    }
+    // tokens of the group
+    const int page = 1 << a.page_shift;
+    const int64_t lo = tok0[0], hi = min(t_end, a.N);
+    for (int64_t i = lo + (int64_t)blockIdx.y * 256 + t; i < hi; i += (int64_t)gridDim.y * 256) {
+        int s = 0;
+        for (int step = MAX_GROUP / 2; step > 0; step >>= 1)   // the last sequence that starts at or before i and holds it
+            if (s + step < nb && tok0[s + step] <= i) s += step;
+        const int64_t p = i - tok0[s], at = page0[s] + (p >> a.page_shift);
+        int32_t slot = -1;
+        if (at < page0[s + 1] && at < a.n_pages) {
+            const int32_t pg = a.pages[at];
+            if (pg >= 0) slot = clip31(((int64_t)pg << a.page_shift) + (p & (page - 1)));
+        }
+        a.slots[i] = slot;
+        a.pos[i] = (int32_t)p;
+        a.seq[i] = (int32_t)(b0 + s);
+    }
+}
+
+__global__ __launch_bounds__(256) void page_step_kernel(const int32_t* __restrict__ base, const int32_t* __restrict__ sent, int64_t t,
+                                                        const int32_t* __restrict__ table, int64_t width, int64_t n_seq, int page_shift,
+                                                        int32_t* __restrict__ slots, int32_t* __restrict__ pos, int32_t* __restrict__ lens,
+                                                        int64_t R) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r >= R) return;
+    const int64_t s = sent != nullptr ? sent[r] : r;
+    int32_t slot = -1, ps = 0, len = 0;
+    if (s >= 0 && s < n_seq) {
+        const int64_t p = (int64_t)max(base[s], 0) + t;
+        ps = clip31(p);
+        len = clip31(p + 1);
+        const int64_t j = p >> page_shift;
+        if (j < width) {
+            const int32_t pg = table[s * width + j];
+            if (pg >= 0) slot = clip31(((int64_t)pg << page_shift) + (p & ((1 << page_shift) - 1)));
+        }
+    }
+    slots[r] = slot;
+    pos[r] = ps;
+    lens[r] = len;
+}
+
+int page_shift_of(int64_t page) {
+    for (int s = 3; s <= 10; ++s)
+        if (page == (int64_t)1 << s) return s;
+    return -1;
+}
+
+}  // namespace
+
+extern "C" int tst_page_plan(const int32_t* lens, const int32_t* room, int64_t B, const int32_t* pages, int64_t n_pages, int64_t page,
+                             int32_t* table, int64_t width, int32_t* cu, int32_t* slots, int32_t* pos, int32_t* seq, int64_t N,
+                             int32_t* used, void* stream) {
+    TST_REQUIRE(tst_dims_ok({B, n_pages, width, N}), TST_ERR_UNSUPPORTED, "tst_page_plan: a size exceeds 2^31 - 1");
+    TST_REQUIRE(B >= 0 && n_pages >= 0 && width >= 0 && N >= 0, TST_ERR_ARG, "tst_page_plan: negative size");
+    const int shift = page_shift_of(page);
+    TST_REQUIRE(shift >= 0, TST_ERR_ARG, "tst_page_plan: page must be a power of two in 8 .. 1024");
+    TST_REQUIRE(cu && used && (B == 0 || lens) && (n_pages == 0 || pages) && (B * width == 0 || table) && (N == 0 || (slots && pos && seq)),
+                TST_ERR_ARG, "tst_page_plan: null pointer");
+    // groups: small enough to spread the writes over the chip, large enough that the sums in front of the groups stay cheap
+    int64_t group = 1;
+    while (group < MAX_GROUP && group * 1024 < B) group *= 2;
+    const int64_t groups = B > 0 ? (B + group - 1) / group : 1;
+    int64_t slices = (N + B * width + groups * 2048 - 1) / (groups * 2048);   // about 8 entries per thread
+    slices = slices < 1 ? 1 : (slices > 1024 ? 1024 : slices);
+    PlanArgs a{lens, room, pages, table, cu, slots, pos, seq, used, B, n_pages, N, width, shift, (int)group};
+    page_plan_kernel<<<dim3((unsigned)groups, (unsigned)slices), 256, 0, (hipStream_t)stream>>>(a);
+    return tst_after_launch("tst_page_plan");
+}
+
+extern "C" int tst_page_step(const int32_t* base, const int32_t* sent, int64_t t, const int32_t* table, int64_t width, int64_t n_seq,
+                             int64_t page, int32_t* slots, int32_t* pos, int32_t* lens, int64_t R, void* stream) {
+    TST_REQUIRE(tst_dims_ok({t, width, n_seq, R}), TST_ERR_UNSUPPORTED, "tst_page_step: a size exceeds 2^31 - 1");
+    TST_REQUIRE(t >= 0 && width >= 0 && n_seq >= 0 && R >= 0, TST_ERR_ARG, "tst_page_step: negative size");
+    const int shift = page_shift_of(page);
+    TST_REQUIRE(shift >= 0, TST_ERR_ARG, "tst_page_step: page must be a power of two in 8 .. 1024");
+    TST_REQUIRE(R == 0 || (slots && pos && lens && (n_seq == 0 || (base && (width == 0 || table)))), TST_ERR_ARG, "tst_page_step: null pointer");
+    if (R == 0) return TST_OK;
+    page_step_kernel<<<(unsigned)((R + 255) / 256), 256, 0, (hipStream_t)stream>>>(base, sent, t, table, width, n_seq, shift, slots, pos, lens, R);
+    return tst_after_launch("tst_page_step");
+}

@@ -2,6 +2,7 @@
 // the selection / retirement tail, each issued from native code in one call, so that small batches are not bound by
 // per-launch interpreter overhead.  Contains no kernels; every launch goes through the entry points of this library.
 #include "tst_common.h"
+#include <math.h>
 
 namespace {
 
@@ -344,4 +345,48 @@ extern "C" int tst_select_step_run(const tst_select_step* s, const tst_rows* cur
     return tst_retire_compact_bounded(cur, nxt, s->sel_parent, s->sel_tok, s->sel_score, s->sel_fin, s->sel_nemit, s->lp, n_sent, s->k, step,
                                       s->T, s->eos, last_step, s->top_ends, s->out_tok, s->out_len, s->out_score, s->scratch_alive_pos,
                                       s->row_parent, s->n_alive, s->n_sent_dev, s->n_alive_host, stream);
+}
+
+extern "C" int tst_paged_step_run(const tst_paged_step* p, const int32_t* tok, const int32_t* sent, int64_t R, int64_t t, void* stream) {
+    TST_REQUIRE(tst_dims_ok({R, t}), TST_ERR_UNSUPPORTED, "tst_paged_step_run: a size exceeds 2^31 - 1");
+    TST_REQUIRE(p != nullptr && p->step != nullptr && p->step->layers != nullptr && p->caches != nullptr, TST_ERR_ARG, "tst_paged_step_run: null plan");
+    const tst_tfm_step* m = p->step;
+    TST_REQUIRE(m->n_layers >= 1 && m->d > 0 && m->heads > 0 && m->d % m->heads == 0 && m->d_ff > 0 && m->V > 0, TST_ERR_ARG,
+                "tst_paged_step_run: bad sizes");
+    TST_REQUIRE(R >= 0 && R <= m->slab_rows, TST_ERR_ARG, "tst_paged_step_run: %lld rows, buffers hold %lld", (long long)R, (long long)m->slab_rows);
+    TST_REQUIRE(t >= 0 && p->max_len >= 1 && p->max_len <= m->n_pos, TST_ERR_ARG, "tst_paged_step_run: max_len outside 1 .. n_pos");
+    TST_REQUIRE(m->x && m->h && m->a && m->ff && m->logits && p->slots && p->pos && p->lens && p->qkv, TST_ERR_ARG, "tst_paged_step_run: null work buffer");
+    TST_REQUIRE(tok && m->emb && m->pe && m->wout && p->base && p->table, TST_ERR_ARG, "tst_paged_step_run: null input");
+    TST_REQUIRE(m->z == nullptr || sent != nullptr, TST_ERR_ARG, "tst_paged_step_run: z without sent");
+    for (int li = 0; li < m->n_layers; ++li) {
+        const tst_tfm_layer& L = m->layers[li];
+        TST_REQUIRE(L.wqkv && L.wo && L.w1 && L.w2 && L.cwq == nullptr, TST_ERR_ARG, "tst_paged_step_run: layer %d incomplete or with cross-attention", li);
+        TST_REQUIRE(p->caches[li].kv_heads == m->heads && p->caches[li].dh * m->heads == m->d && p->caches[li].page == p->caches[0].page, TST_ERR_ARG,
+                    "tst_paged_step_run: the cache of layer %d does not fit the model", li);
+    }
+    if (R == 0) return TST_OK;
+    const int64_t d = m->d, esz = m->bf16 != 0 ? 2 : 4;
+    const StepCtx c{m, R, stream, m->bf16 != 0};
+    TST_TRY(tst_page_step(p->base, sent, t, p->table, p->width, p->n_seq, p->caches[0].page, p->slots, p->pos, p->lens, R, stream));
+    if (m->z != nullptr) TST_TRY(tst_embed_posadd_rows_f32(tok, m->emb, m->pe, p->pos, m->scale, m->z, sent, m->x, R, d, m->V, stream));
+    else TST_TRY(tst_embed_posadd_f32(tok, m->emb, m->pe, p->pos, m->scale, m->x, R, d, m->V, stream));
+    const float scale = (float)(1.0 / sqrt((double)(d / m->heads)));
+    char* qkv = (char*)p->qkv;
+    for (int li = 0; li < m->n_layers; ++li) {
+        const tst_tfm_layer& L = m->layers[li];
+        const tst_cache4* cache = p->caches + li;
+        TST_TRY(c.ln_gemm(L.ln_self_g, L.ln_self_b, L.wqkv, L.ld_wqkv, L.bqkv, qkv, 3 * d, 3 * d, 0));
+        TST_TRY(c.bf16 ? tst_cache4_write_bf16(cache, qkv + d * esz, 3 * d, qkv + 2 * d * esz, 3 * d, p->slots, R, stream)
+                       : tst_cache4_write_f32(cache, (const float*)(qkv + d * esz), 3 * d, (const float*)(qkv + 2 * d * esz), 3 * d, p->slots, R,
+                                              stream));
+        TST_TRY(c.bf16 ? tst_attn_cache4_bf16(cache, qkv, 3 * d, p->table, p->width, p->n_seq, sent, p->lens, p->max_len, m->a, d, R, m->heads,
+                                              scale, p->work, p->n_work, stream)
+                       : tst_attn_cache4_f32(cache, (const float*)qkv, 3 * d, p->table, p->width, p->n_seq, sent, p->lens, p->max_len,
+                                             (float*)m->a, d, R, m->heads, scale, p->work, p->n_work, stream));
+        TST_TRY(c.gemm(m->a, d, L.wo, L.ld_wo, L.bo, m->x, d, m->x, d, d, d, 0, false));
+        TST_TRY(c.ln_gemm(L.ln_ff_g, L.ln_ff_b, L.w1, L.ld_w1, L.b1, m->ff, m->d_ff, m->d_ff, 1));
+        TST_TRY(c.gemm(m->ff, m->d_ff, L.w2, L.ld_w2, L.b2, m->x, d, m->x, d, d, m->d_ff, 0, false));
+    }
+    TST_TRY(c.layernorm(m->x, m->ln_g, m->ln_b, m->h));
+    return c.gemm(m->h, d, m->wout, m->ld_wout, m->bout, nullptr, 0, m->logits, m->ld_logits, m->V, d, 0, true);
 }
