@@ -13,7 +13,10 @@ pids=()
 for f in $UNITS; do
   if [ ! -f $f.o ] || [ $f.hip -nt $f.o ] || [ build.sh -nt $f.o ] || [ tst_common.h -nt $f.o ] || [ ../../include/tst_hip.h -nt $f.o ]; then
     rm -f $f.o
-    /opt/rocm/bin/hipcc $FLAGS -c $f.hip -o $f.o &
+    EXTRA=""
+    # the attention kernels do vector arithmetic on matrix accumulators all the time: keep those in ordinary registers
+    case $f in cache4|prompt) EXTRA="-mllvm -amdgpu-mfma-vgpr-form=1" ;; esac
+    /opt/rocm/bin/hipcc $FLAGS $EXTRA -c $f.hip -o $f.o &
     pids+=($!)
   fi
 done

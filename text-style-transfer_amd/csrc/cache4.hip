@@ -102,84 +102,452 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Cache c, const int32_t
     }
 }
 
-// One wave per (row, head): 64 tokens at a time, one per lane for the scores, then each lane sums its elements of the head over
-// them with the running maximum and sum of the softmax.
-template <typename T>
-__global__ __launch_bounds__(64) void attn_cache4_kernel(Cache c, const T* __restrict__ q, int64_t ldq, const int32_t* __restrict__ table,
-                                                         int64_t width, int64_t n_seq, const int32_t* __restrict__ seq,
-                                                         const int32_t* __restrict__ lens, int64_t max_len, T* __restrict__ out,
-                                                         int64_t ldo, int heads, float scale) {
-    __shared__ float qs[256], ws[64];
-    __shared__ int64_t at[64];
-    const int lane = threadIdx.x;
-    const int64_t r = blockIdx.x / heads;
-    const int h = (int)(blockIdx.x - r * heads), g = h / (heads / c.kv_heads);
-    const int dh = c.dh, groups = dh >> 5, page = 1 << c.page_shift;
-    const int64_t s = seq != nullptr ? seq[r] : r;
-    int64_t len = s >= 0 && s < n_seq ? lens[r] : 0;
-    len = min(min(len, max_len), width * page);
-    for (int e = lane; e < dh; e += 64) qs[e] = load1(q + r * ldq + h * dh + e);
-    __syncthreads();
-    bool any = false;
-    float m = -INFINITY, sum = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t p0 = 0; p0 < len; p0 += 64) {
-        const int64_t p = p0 + lane;
-        float score = -INFINITY;
-        int64_t slot = -1;
-        if (p < len) {
-            const int32_t pg = table[s * width + (p >> c.page_shift)];
-            if (pg >= 0 && ((int64_t)pg << c.page_shift) < c.slots) slot = ((int64_t)pg << c.page_shift) + (p & (page - 1));
-        }
-        if (slot >= 0) {
-            const int64_t row = ((slot >> c.page_shift) * c.kv_heads + g) * page + (slot & (page - 1));
-            float a = 0.0f;
-            for (int w = 0; w < groups; ++w) {
-                const float f = scale_of(c.ks[row * groups + w]);
-                for (int e = 0; e < 16; ++e) {
-                    const uint32_t b = c.kc[row * (dh >> 1) + w * 16 + e];
-                    a = __builtin_fmaf(qs[w * 32 + 2 * e], value_of(b & 15u) * f, a);
-                    a = __builtin_fmaf(qs[w * 32 + 2 * e + 1], value_of(b >> 4) * f, a);
-                }
-            }
-            score = a * scale;
-        }
-        at[lane] = slot;
-        const unsigned long long live = __ballot(slot >= 0);
-        if (live == 0ull) continue;
-        any = true;
-        // a NaN score has to reach the result: fmax would drop it
-        const unsigned long long nan = __ballot(slot >= 0 && score != score);
-        float top = score;
-        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-        const float mn = nan != 0ull ? __builtin_nanf("") : fmaxf(m, top);
-        const float w = slot >= 0 && mn != -INFINITY ? __expf(score - mn) : 0.0f;
-        const float keep = m == -INFINITY ? 0.0f : __expf(m - mn);
-        float total = w;
-        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
-        sum = sum * keep + total;
-        m = mn;
-        ws[lane] = w;
-        __syncthreads();
-        for (int u = 0; u < 4; ++u) {
-            const int e = lane + 64 * u;
-            if (e < dh) {
-                acc[u] *= keep;
-                for (int j = 0; j < 64; ++j) {
-                    if (at[j] < 0) continue;
-                    const int64_t ph = (at[j] >> c.page_shift) * c.kv_heads + g;
-                    const int tok = (int)(at[j] & (page - 1));
-                    const uint32_t b = c.vc[(ph * (dh >> 1) + (e >> 1)) * page + tok];
-                    const float f = scale_of(c.vs[(ph * groups + (e >> 5)) * page + tok]);
-                    acc[u] = __builtin_fmaf(ws[j], value_of((e & 1) != 0 ? b >> 4 : b & 15u) * f, acc[u]);
-                }
-            }
-        }
-        __syncthreads();
+// ---- attention of single query rows over the cache -----------------------------------------------------------------------------
+//
+// A wave takes one (row, key head) and walks tiles of 64 tokens; the up to 16 query heads that share the key head are the columns of
+// its matrix products, so they cost no further reads.  Per tile, on v_mfma_f32_16x16x32_bf16:
+//     S^T [64 tokens x 16 heads] = K [64 x dh] Q^T           four products of 16 tokens
+//     O^T [dh x 16 heads]       += V^T [dh x 64] P^T
+// Codes become bf16 (exactly) with v_cvt_scalef32_pk_bf16_fp4, which also applies the group's power of two.  The contraction index of
+// a product may be permuted if both operands agree, and the layout uses that twice so that nothing ever crosses lanes:
+//   - lane quarter j (lane >> 4) loads the dh / 4 adjacent elements j dh / 4 .. of its token's key in one piece (for dh = 128 one 16-byte
+//     load and one scale) and calls them its share of the contraction; the query is laid out to match.
+//   - row 4 a + i of product u is token 16 a + 4 u + i, so the accumulators of quarter j hold the scores of the 16 adjacent tokens 16 j ..
+//     after the four products: exactly the tokens whose value codes quarter j loads as 16 adjacent bytes.
+// Running maximum and sum are per lane (one head each); the maximum is shared by the four quarters through two lane exchanges, the sum
+// only at the end.  fp32 queries and weights enter as three bf16 pieces (8 + 8 + 8 bits of significand), the codes being exact: fp32
+// accuracy at three matrix instructions instead of one.  bf16 queries are one piece, and the weights are rounded to bf16 (half a step,
+// 2^-9 of a weight in [2^k, 2^(k+1)), against an output of 8 bits).
+//
+// Long contexts are split over workgroups (rows x key heads x chunks) and, inside one, over its waves (tile by tile in turn); partial
+// (maximum, sum, O) are joined in LDS and by combine_kernel, in a fixed order.
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+union Frag {
+    uint32_t u[4];
+    bf16x8 v;
+};
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const bf16x2 v = __builtin_convertvector(f32x2{a, b}, bf16x2);
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ float low_f(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high_f(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
+__device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpret_cast<f32x2*>(p) = f32x2{a, b}; }
+__device__ __forceinline__ void store2(__bf16* p, float a, float b) { *reinterpret_cast<uint32_t*>(p) = pack2(a, b); }
+
+// two floats as NP bf16 pieces each: piece i rounds what the pieces before it left
+template <int NP>
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&p)[NP]) {
+    p[0] = pack2(a, b);
+#pragma unroll
+    for (int i = 1; i < NP; ++i) {
+        a -= low_f(p[i - 1]);
+        b -= high_f(p[i - 1]);
+        p[i] = pack2(a, b);
     }
+}
+
+// elements 2 SEL, 2 SEL + 1 of a word of codes; the conversion reads bits 23 .. 30 of the scale only
+template <int SEL>
+__device__ __forceinline__ uint32_t cvt4(uint32_t codes, uint32_t scale_bits) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, __uint_as_float(scale_bits), SEL));
+}
+// byte b of a word of scales, moved to bits 23 .. 30
+__device__ __forceinline__ uint32_t scale_bits(uint32_t w, int b) { return b == 0 ? w << 23 : (b == 1 ? w << 15 : (b == 2 ? w << 7 : w >> 1)); }
+
+struct AttendArgs {
+    Cache c;
+    const void* q;
+    int64_t ldq, width, n_seq, max_len, ldo, R;
+    const int32_t *table, *seq, *lens;
+    void* out;
+    float* work;
+    int heads, per_kv, head_groups, splits, chunk;
+    float scale2;       // |scale| * log2(e), never 0: scores are compared before they are scaled
+    int negate;         // the scale is negative: the query changes its sign
+};
+
+// The pages of a lane's tokens in the tile at p0: 16 adjacent tokens are in one page; the key rows of a lane are in block (lane & 15) >> 2
+// of the tile, its values in block lane >> 4.  Read one tile ahead, so that a tile's loads do not wait for the table.
+struct Pages {
+    int k, v;
+};
+__device__ __forceinline__ Pages load_pages(const int32_t* __restrict__ row_table, int page_shift, int p0, int last, int lane) {
+    return Pages{row_table[min(p0 + 16 * ((lane & 15) >> 2), last) >> page_shift], row_table[min(p0 + 16 * (lane >> 4), last) >> page_shift]};
+}
+
+// key codes and scales of the lane's token of each of the four products
+template <int DH>
+struct KeyTile {
+    uint32_t c[4][DH / 32], s[4];
+};
+template <int DH>
+__device__ __forceinline__ void load_keys(KeyTile<DH>& t, const Cache& c, int pk, int p0, int g, int lane) {
+    const int m = lane & 15, j = lane >> 4, page = 1 << c.page_shift;
+    pk = (unsigned)pk < (unsigned)(c.slots >> c.page_shift) ? pk : 0;     // a page that does not exist: any page, its tokens count as nothing
+    const int64_t row = ((int64_t)pk * c.kv_heads + g) * page + ((p0 + 16 * (m >> 2)) & (page - 1)) + (m & 3);
+    const uint8_t* kc = c.kc + row * (DH / 2) + j * (DH / 8);
+    const uint8_t* ks = c.ks + row * (DH / 32);
+#pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const int e = lane + 64 * u;
-        if (e < dh) store1(out + r * ldo + h * dh + e, any ? acc[u] / sum : 0.0f);
+        const uint8_t* p = kc + u * 4 * (DH / 2);
+        if (DH == 32) t.c[u][0] = *reinterpret_cast<const uint32_t*>(p);
+        if (DH == 64) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            t.c[u][0] = x.x; t.c[u][1 % (DH / 32)] = x.y;
+        }
+        if (DH >= 128) {
+#pragma unroll
+            for (int q = 0; q < DH / 128; ++q) {
+                const uint4 x = reinterpret_cast<const uint4*>(p)[q];
+                t.c[u][4 * q % (DH / 32)] = x.x; t.c[u][(4 * q + 1) % (DH / 32)] = x.y;
+                t.c[u][(4 * q + 2) % (DH / 32)] = x.z; t.c[u][(4 * q + 3) % (DH / 32)] = x.w;
+            }
+        }
+        const uint8_t* s = ks + u * 4 * (DH / 32);
+        if (DH == 256) t.s[u] = *reinterpret_cast<const uint16_t*>(s + 2 * j);
+        else t.s[u] = s[DH == 128 ? j : (DH == 64 ? j >> 1 : 0)];
     }
+}
+
+// Value codes and scales of the 16 tokens of the lane's quarter.  Row m of the output tiles is spread over the head so that all pieces of a
+// lane are of one group of 32 elements (one scale per token): with G groups and 16 / G rows for each, piece b of row m is byte row
+// 16 (m / (16 / G)) + (16 / G) b + m % (16 / G), i.e. elements 2 x and 2 x + 1 of that byte row x.
+template <int DH>
+struct ValueTile {
+    uint32_t c[DH / 32][4], s[4];
+    int live;           // how many of the tokens count (0 .. 16)
+};
+template <int DH>
+__device__ __forceinline__ int value_row(int m, int b) {
+    constexpr int L = 512 / DH;       // 16 / G
+    return 16 * (m / L) + L * b + m % L;
+}
+template <int DH>
+__device__ __forceinline__ void load_values(ValueTile<DH>& t, const Cache& c, int pv, int p0, int len, int g, int lane) {
+    constexpr int L = 512 / DH;
+    const int m = lane & 15, page = 1 << c.page_shift;
+    const bool ok = (unsigned)pv < (unsigned)(c.slots >> c.page_shift);
+    const int tv = p0 + 16 * (lane >> 4);
+    t.live = ok ? max(0, min(16, len - tv)) : 0;
+    const int64_t hv = (int64_t)(ok ? pv : 0) * c.kv_heads + g;
+    const int iv = tv & (page - 1);
+    const uint8_t* vc = c.vc + ((hv * (DH / 2) + value_row<DH>(m, 0)) << c.page_shift) + iv;
+    const uint4 y = *reinterpret_cast<const uint4*>(c.vs + ((hv * (DH / 32) + m / L) << c.page_shift) + iv);
+    t.s[0] = y.x; t.s[1] = y.y; t.s[2] = y.z; t.s[3] = y.w;
+#pragma unroll
+    for (int b = 0; b < DH / 32; ++b) {
+        const uint4 x = *reinterpret_cast<const uint4*>(vc + ((L * b) << c.page_shift));
+        t.c[b][0] = x.x; t.c[b][1] = x.y; t.c[b][2] = x.z; t.c[b][3] = x.w;
+    }
+}
+
+template <typename T, int DH, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attn_cache4_kernel(AttendArgs a) {
+    constexpr int NP = sizeof(T) == 4 ? 3 : 1;     // bf16 pieces of a query element or weight
+    constexpr int KS = DH / 32;                    // steps of a key product
+    constexpr int MT = DH / 16;                    // output tiles of 16 elements
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int n = lane & 15, j = lane >> 4;
+    uint32_t id = blockIdx.x;                      // (chunk, row, key head, group of 16 heads)
+    const int hg = (int)(id % (uint32_t)a.head_groups);
+    id /= (uint32_t)a.head_groups;
+    const int g = (int)(id % (uint32_t)a.c.kv_heads);
+    id /= (uint32_t)a.c.kv_heads;
+    const int64_t r = id % (uint32_t)a.R;
+    const int split = (int)(id / (uint32_t)a.R);
+
+    const int64_t s = a.seq != nullptr ? a.seq[r] : r;
+    int64_t len = s >= 0 && s < a.n_seq ? a.lens[r] : 0;
+    len = max(min(min(len, a.max_len), a.width << a.c.page_shift), (int64_t)0);
+    if (split > 0 && (int64_t)split * a.chunk >= len) return;      // the whole workgroup: nothing here, combine_kernel knows
+    const int lo = split * a.chunk, hi = (int)min(len, (int64_t)lo + a.chunk);
+    const int32_t* row_table = a.table + s * a.width;
+    const int col = hg * 16 + n;                   // head of the group this lane's column stands for
+    const bool real = col < a.per_kv;
+    const int64_t head = (int64_t)g * a.per_kv + col;
+
+    // the query as the B operand: column n, this quarter's dh / 4 elements, 8 per step
+    uint32_t q[KS][NP][4];
+    {
+        const T* qp = (const T*)a.q + r * a.ldq + (real ? head : 0) * DH + j * (DH / 4);
+#pragma unroll
+        for (int st = 0; st < KS; ++st)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x = load1(qp + st * 8 + 2 * e), y = load1(qp + st * 8 + 2 * e + 1);
+                if (!real) { x = 0.0f; y = 0.0f; }
+                if (a.negate) { x = -x; y = -y; }
+                uint32_t p[NP];
+                split2<NP>(x, y, p);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) q[st][i][e] = p[i];
+            }
+    }
+    f32x4 o[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, sum = 0.0f;
+    bool any = false;
+
+    int p0 = lo + 64 * w;
+    // in flight while a tile is computed: its values during the scores, the next tile's keys during the rest
+    KeyTile<DH> keys;
+    Pages at, next;
+    if (p0 < hi) {
+        at = load_pages(row_table, a.c.page_shift, p0, hi - 1, lane);
+        next = load_pages(row_table, a.c.page_shift, p0 + 64 * WAVES, hi - 1, lane);
+        load_keys<DH>(keys, a.c, at.k, p0, g, lane);
+    }
+    for (; p0 < hi; p0 += 64 * WAVES) {
+        ValueTile<DH> cur;
+        load_values<DH>(cur, a.c, at.v, p0, hi, g, lane);
+        const unsigned long long full = __ballot(cur.live == 16);
+        // scores of this lane's head for the 16 tokens of its quarter: sc[u][i] is token 4 u + i
+        f32x4 sc[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < KS; ++st) {
+                const uint32_t word = keys.c[u][st];
+                const uint32_t f = DH == 256 && st >= 4 ? keys.s[u] << 15 : keys.s[u] << 23;
+                Frag k;
+                k.u[0] = cvt4<0>(word, f); k.u[1] = cvt4<1>(word, f); k.u[2] = cvt4<2>(word, f); k.u[3] = cvt4<3>(word, f);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    Frag qq;
+                    qq.u[0] = q[st][i][0]; qq.u[1] = q[st][i][1]; qq.u[2] = q[st][i][2]; qq.u[3] = q[st][i][3];
+                    sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k.v, qq.v, sc[u], 0, 0, 0);
+                }
+            }
+        }
+        at = next;
+        if (p0 + 64 * WAVES < hi) {
+            load_keys<DH>(keys, a.c, at.k, p0 + 64 * WAVES, g, lane);
+            next = load_pages(row_table, a.c.page_shift, p0 + 128 * WAVES, hi - 1, lane);
+        }
+        if (full != ~0ull) {   // the end of the context, or a page that does not exist
+            any |= __ballot(cur.live > 0) != 0ull;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int left = min(max(cur.live - 4 * u, 0), 4);
+                const uint32_t keep = left == 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
+                cur.s[u] &= keep;
+#pragma unroll
+                for (int b = 0; b < DH / 32; ++b) cur.c[b][u] &= keep;      // value 0, whatever the page holds there
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[u][i] = i < left ? sc[u][i] : -INFINITY;
+            }
+        } else {
+            any = true;
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[u][i]);
+        top = fmaxf(top, lane_xor<16>(top));
+        top = fmaxf(top, lane_xor<32>(top));
+        const float base = top == -INFINITY ? 0.0f : top * a.scale2;       // no finite score yet: every weight is exp(-inf) = 0
+        if (__ballot(top != m) != 0ull) {
+            const float keep = __builtin_amdgcn_exp2f(__builtin_fmaf(m, a.scale2, -base));     // m = -inf: 0
+            sum *= keep;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) o[t] = o[t] * keep;
+            m = top;
+        }
+        // the weights as the B operand: step st holds tokens 8 st .. 8 st + 7 of the quarter
+        uint32_t p[2][NP][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], a.scale2, -base));
+                sum += e[i];
+            }
+            uint32_t x[NP], y[NP];
+            split2<NP>(e[0], e[1], x);
+            split2<NP>(e[2], e[3], y);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) { p[u >> 1][i][2 * (u & 1)] = x[i]; p[u >> 1][i][2 * (u & 1) + 1] = y[i]; }
+        }
+#pragma unroll
+        for (int b = 0; b < DH / 32; ++b) {
+            // 16 tokens of the even and of the odd element of this piece's byte row
+            Frag even[2], odd[2];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint32_t word = cur.c[b][u], f = cur.s[u];
+                const uint32_t t0 = cvt4<0>(word, scale_bits(f, 0)), t1 = cvt4<1>(word, scale_bits(f, 1));
+                const uint32_t t2 = cvt4<2>(word, scale_bits(f, 2)), t3 = cvt4<3>(word, scale_bits(f, 3));
+                even[u >> 1].u[2 * (u & 1)] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
+                even[u >> 1].u[2 * (u & 1) + 1] = __builtin_amdgcn_perm(t3, t2, 0x05040100u);
+                odd[u >> 1].u[2 * (u & 1)] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
+                odd[u >> 1].u[2 * (u & 1) + 1] = __builtin_amdgcn_perm(t3, t2, 0x07060302u);
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    Frag pp;
+                    pp.u[0] = p[st][i][0]; pp.u[1] = p[st][i][1]; pp.u[2] = p[st][i][2]; pp.u[3] = p[st][i][3];
+                    o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even[st].v, pp.v, o[2 * b], 0, 0, 0);
+                    o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd[st].v, pp.v, o[2 * b + 1], 0, 0, 0);
+                }
+        }
+    }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (!any) sum = -1.0f;                          // nothing to attend to (a sum of weights is never negative)
+
+    // join the waves: o[2 b + x][i] is element 2 * value_row(4 j + i, b) + x of head n; the maximum becomes one of scaled scores
+    m *= a.scale2;
+    if (WAVES > 1) {
+        __shared__ float red[WAVES][16][2];
+        __shared__ float part[WAVES > 1 ? WAVES - 1 : 1][DH][17];
+        if (j == 0) { red[w][n][0] = m; red[w][n][1] = sum; }
+        __syncthreads();
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) top = fmaxf(top, red[i][n][1] < 0.0f ? -INFINITY : red[i][n][0]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float total = 0.0f;
+        bool some = false;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i)
+            if (!(red[i][n][1] < 0.0f)) {
+                total += red[i][n][1] * __builtin_amdgcn_exp2f(red[i][n][0] - base);
+                some = true;
+            }
+        const float mine = sum < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - base);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) o[t] = o[t] * mine;
+        if (w > 0) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[w - 1][4 * MT * j + 4 * t + i][n] = o[t][i];
+        }
+        __syncthreads();
+        if (w > 0) return;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int x = 0; x < WAVES - 1; ++x) o[t][i] += part[x][4 * MT * j + 4 * t + i][n];
+        m = top;
+        sum = some ? total : -1.0f;
+    }
+    if (!real) return;
+    if (len <= a.chunk) {                           // the whole row is here
+        const float inv = sum < 0.0f ? 0.0f : 1.0f / sum;
+        T* op = (T*)a.out + r * a.ldo + head * DH;
+#pragma unroll
+        for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                store2(op + 2 * value_row<DH>(4 * j + i, b), sum < 0.0f ? 0.0f : o[2 * b][i] * inv, sum < 0.0f ? 0.0f : o[2 * b + 1][i] * inv);
+    } else {
+        const int64_t at = (r * a.heads + head) * a.splits + split;
+        float* ml = a.work + 2 * at;
+        float* op = a.work + 2 * a.R * a.heads * a.splits + at * DH;
+        if (j == 0) { ml[0] = m; ml[1] = sum; }
+#pragma unroll
+        for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) store2(op + 2 * value_row<DH>(4 * j + i, b), o[2 * b][i], o[2 * b + 1][i]);
+    }
+}
+
+// Joins the chunks of the rows that have more than one: one workgroup per (row, head), its eight waves take every eighth chunk, lane = up to
+// 4 adjacent elements.
+template <typename T, int DH>
+__global__ __launch_bounds__(512) void attn_cache4_combine_kernel(AttendArgs a) {
+    constexpr int E = DH <= 64 ? 1 : DH / 64;
+    __shared__ float part[8][64 * E + 1];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t r = blockIdx.x / (uint32_t)a.heads, head = blockIdx.x - r * a.heads;
+    const int64_t s = a.seq != nullptr ? a.seq[r] : r;
+    int64_t len = s >= 0 && s < a.n_seq ? a.lens[r] : 0;
+    len = max(min(min(len, a.max_len), a.width << a.c.page_shift), (int64_t)0);
+    if (len <= a.chunk) return;
+    const int n = (int)((len + a.chunk - 1) / a.chunk);
+    const float* ml = a.work + 2 * (r * a.heads + head) * a.splits;
+    const float* op = a.work + 2 * a.R * a.heads * a.splits + (r * a.heads + head) * a.splits * DH;
+    float m = -INFINITY;
+    bool some = false;
+    for (int i = lane; i < n; i += 64)
+        if (!(ml[2 * i + 1] < 0.0f)) { m = fmaxf(m, ml[2 * i]); some = true; }
+    m = wave_max(m);
+    some = __ballot(some) != 0ull;
+    const float base = m == -INFINITY ? 0.0f : m;
+    float acc[E], sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+#pragma unroll 4
+    for (int i = w; i < n; i += 8) {
+        const float si = ml[2 * i + 1];
+        const float f = si < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * i] - base);
+        sum += si < 0.0f ? 0.0f : si * f;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (lane * E + e < DH) acc[e] += op[(int64_t)i * DH + lane * E + e] * f;    // a chunk without tokens holds zeros
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[w][lane * E + e] = acc[e];
+    if (lane == 0) part[w][64 * E] = sum;
+    __syncthreads();
+    if (w > 0) return;
+    sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) sum += part[x][64 * E];
+    T* out = (T*)a.out + r * a.ldo + head * DH;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = lane * E + e;
+        float total = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) total += part[x][i];
+        if (i < DH) store1(out + i, some ? total / sum : 0.0f);
+    }
+}
+
+// How a call is cut: tokens per workgroup (chunk) and how many chunks the longest row may have.  Few (row, key head) units: as many
+// workgroups as run at once, two to a CU, since every chunk costs a prologue and a partial result (3 rows x 4 key heads, 131001
+// tokens: 38.8 us at 512 workgroups, 41.5 at 1024, 46.7 at 1536).  Many: 1024, so that rows of different lengths even out, and whole
+// rows up to 8192 tokens once there are that many units (256 rows x 8 key heads, up to 8000 tokens: 219 us in one piece, 225 cut at
+// 4096, 231 at 2048).  At least one tile for each of the four waves.
+void cut(int64_t R, int64_t kv_heads, int64_t head_groups, int64_t max_len, int* chunk, int* splits) {
+    const int64_t units = R * kv_heads * head_groups, target = units < 128 ? 512 : 1024;
+    int64_t c = (max_len * units + target - 1) / target;
+    c = (c + 255) / 256 * 256;
+    c = c < 256 ? 256 : (c > 8192 ? 8192 : c);
+    *chunk = (int)c;
+    *splits = max_len > 0 ? (int)((max_len + c - 1) / c) : 1;
+}
+
+template <typename T, int DH>
+int launch_attend(const AttendArgs& a, hipStream_t st, const char* who) {
+    const int64_t groups = a.R * a.c.kv_heads * a.head_groups * a.splits;
+    TST_REQUIRE(groups <= (int64_t)0x7fffffff, TST_ERR_UNSUPPORTED, "%s: rows * heads exceeds 2^31 - 1", who);
+    if (a.max_len <= 64) attn_cache4_kernel<T, DH, 1><<<(unsigned)groups, 64, 0, st>>>(a);
+    else attn_cache4_kernel<T, DH, 4><<<(unsigned)groups, 256, 0, st>>>(a);
+    int rc = tst_after_launch(who);
+    if (rc == TST_OK && a.splits > 1) {
+        attn_cache4_combine_kernel<T, DH><<<(unsigned)(a.R * a.heads), 512, 0, st>>>(a);
+        rc = tst_after_launch(who);
+    }
+    return rc;
 }
 
 int check_cache(const tst_cache4* c, Cache* o, const char* who) {
@@ -252,9 +620,15 @@ int attn_cache4(const tst_cache4* c, const T* q, int64_t ldq, const int32_t* tab
                 (long long)n_work, (long long)need);
     if (R == 0) return TST_OK;
     TST_REQUIRE(R * heads <= (int64_t)0x7fffffff, TST_ERR_UNSUPPORTED, "%s: rows * heads exceeds 2^31 - 1", who);
-    attn_cache4_kernel<T><<<(unsigned)(R * heads), 64, 0, (hipStream_t)stream>>>(d, q, ldq, table, width, n_seq, seq, lens, max_len, out, ldo,
-                                                                                 (int)heads, scale);
-    return tst_after_launch(who);
+    if (d.slots == 0 || width == 0 || n_seq == 0) max_len = 0;     // nothing can be attended to: zeros
+    AttendArgs a{d, q, ldq, width, n_seq, max_len, ldo, R, table, seq, lens, out, work, (int)heads, (int)(heads / d.kv_heads),
+                 (int)((heads / d.kv_heads + 15) / 16), 1, 0, fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-37f), scale < 0.0f ? 1 : 0};
+    cut(R, d.kv_heads, a.head_groups, max_len, &a.chunk, &a.splits);
+    hipStream_t st = (hipStream_t)stream;
+    if (d.dh == 32) return launch_attend<T, 32>(a, st, who);
+    if (d.dh == 64) return launch_attend<T, 64>(a, st, who);
+    if (d.dh == 128) return launch_attend<T, 128>(a, st, who);
+    return launch_attend<T, 256>(a, st, who);
 }
 
 }  // namespace
@@ -277,8 +651,10 @@ extern "C" int tst_cache4_read_bf16(const tst_cache4* c, const int32_t* slots, v
 }
 
 extern "C" int64_t tst_attn_cache4_work(int64_t R, int64_t heads, int64_t kv_heads, int64_t dh, int64_t max_len) {
-    (void)R; (void)heads; (void)kv_heads; (void)dh; (void)max_len;
-    return 0;
+    if (R < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dh < 1 || max_len < 0 || !tst_dims_ok({R, heads, dh, max_len})) return -1;
+    int chunk, splits;
+    cut(R, kv_heads, (heads / kv_heads + 15) / 16, max_len, &chunk, &splits);
+    return splits > 1 ? R * heads * splits * (dh + 2) : 0;
 }
 extern "C" int tst_attn_cache4_f32(const tst_cache4* c, const float* q, int64_t ldq, const int32_t* table, int64_t width, int64_t n_seq,
                                    const int32_t* seq, const int32_t* lens, int64_t max_len, float* out, int64_t ldo, int64_t R,
