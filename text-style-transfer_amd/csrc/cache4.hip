@@ -25,80 +25,185 @@ __device__ __forceinline__ int scale_byte(uint32_t top_bits) {
     const int s = (int)(top_bits >> 23) - 2 + ((top_bits & 0x7fffffu) > 0x400000u ? 1 : 0);
     return s < 1 ? 1 : s;
 }
-// 2^-(s - 127) as a float, s in 1 .. 253
-__device__ __forceinline__ float inverse_scale(int s) { return __uint_as_float((uint32_t)(254 - s) << 23); }
+__device__ __forceinline__ uint32_t scale_to_bits(int s) { return (uint32_t)s << 23; }
 
-// the code of y = x * 2^-E, |y| <= 6: nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, ties to the even code
-__device__ __forceinline__ uint32_t code_of(float y) {
-    const float a = fabsf(y);
-    const uint32_t m = (uint32_t)(a > 0.25f) + (uint32_t)(a >= 0.75f) + (uint32_t)(a > 1.25f) + (uint32_t)(a >= 1.75f) +
-                       (uint32_t)(a > 2.5f) + (uint32_t)(a >= 3.5f) + (uint32_t)(a > 5.0f);
-    return m | (y < 0.0f ? 8u : 0u);
-}
-// the value of a code
-__device__ __forceinline__ float value_of(uint32_t c) {
-    const uint32_t e = (c >> 1) & 3u, m = c & 1u;
-    const float v = e == 0u ? (m != 0u ? 0.5f : 0.0f) : __uint_as_float(((e + 126u) << 23) | (m << 22));
-    return (c & 8u) != 0u ? -v : v;
-}
-__device__ __forceinline__ float scale_of(uint32_t s) { return s == 255u ? __builtin_nanf("") : __uint_as_float((s < 1u ? 1u : s) << 23); }
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// One lane per (token, group of 32 elements): lanes of a wave are consecutive tokens, so that the bytes of the token-minor value
-// codes are written side by side; the 4 waves of a workgroup take 4 adjacent groups of the same 64 tokens.
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const bf16x2 v = __builtin_convertvector(f32x2{a, b}, bf16x2);
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ float low_f(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high_f(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
+// elements 2 SEL, 2 SEL + 1 of a word of codes; the conversion reads bits 23 .. 30 of the scale only, and gives NaN for scale byte 255
+template <int SEL>
+__device__ __forceinline__ uint32_t cvt4(uint32_t codes, uint32_t scale_bits) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, __uint_as_float(scale_bits), SEL));
+}
+template <int SEL>
+__device__ __forceinline__ f32x2 cvt4f(uint32_t codes, uint32_t scale_bits) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, __uint_as_float(scale_bits), SEL);
+}
+
+// ---- storing and reading back ---------------------------------------------------------------------------------------------------
+//
+// A workgroup takes 64 rows x 128 elements (4 groups).  Memory sees whole rows of the tile, 16 bytes per lane side by side; between
+// that and the codes the tile passes through LDS, from where each lane (= row) of a wave (= group) reads its 32 elements (rows padded
+// by 16 bytes: 16 lanes fall on 16 different 16-byte places).  Key codes leave as 16 bytes per lane.  Value codes lie token by token:
+// where the four rows of a lane quad have adjacent slots, the quad transposes its bytes and every lane writes words of four tokens
+// (at any byte address), else single bytes.
+
+constexpr int TILE_ROWS = 64, TILE_COLS = 128;
+
+template <typename T>
+struct RowTile {
+    static constexpr int ROW_BYTES = TILE_COLS * (int)sizeof(T) + 16;
+    static constexpr int CHUNKS = TILE_COLS * (int)sizeof(T) / 16;       // 16-byte pieces per row
+};
+
+struct __attribute__((packed, aligned(1))) word_any {
+    uint32_t v;
+};
+
+// 4 x 4 bytes across the four lanes of a quad: byte b of lane q becomes byte q of lane b
+__device__ __forceinline__ uint32_t quad_transpose(uint32_t x, int q) {
+    const uint32_t y = (uint32_t)lane_xor_i<1>((int)x);
+    x = __builtin_amdgcn_perm(y, x, (q & 1) != 0 ? 0x03070105u : 0x06020400u);
+    const uint32_t z = (uint32_t)lane_xor_i<2>((int)x);
+    return __builtin_amdgcn_perm(z, x, (q & 2) != 0 ? 0x03020706u : 0x05040100u);
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void cache4_write_kernel(Cache c, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v,
                                                            int64_t ldv, const int32_t* __restrict__ slots, int64_t n) {
-    const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int groups = c.dh >> 5;
-    const int hg = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (i >= n || hg >= c.kv_heads * groups) return;
-    const int64_t slot = slots[i];
-    if (slot < 0 || slot >= c.slots) return;
-    const int h = hg / groups, g = hg - h * groups;
-    const int page = 1 << c.page_shift;
-    const int64_t ph = (slot >> c.page_shift) * c.kv_heads + h;
-    const int tok = (int)(slot & (page - 1));
-    const T* src = (blockIdx.z == 0 ? k + i * ldk : v + i * ldv) + h * c.dh + g * 32;
-    float x[32];
-    uint32_t top = 0;
-    for (int e = 0; e < 32; ++e) {
-        x[e] = load1(src + e);
-        const uint32_t a = __float_as_uint(x[e]) & 0x7fffffffu;
-        top = top > a ? top : a;
+    __shared__ __attribute__((aligned(16))) unsigned char tile[TILE_ROWS * RowTile<T>::ROW_BYTES];
+    constexpr int E = 16 / (int)sizeof(T), CHUNKS = RowTile<T>::CHUNKS;
+    const bool is_v = blockIdx.z != 0;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t i0 = (int64_t)blockIdx.x * TILE_ROWS;
+    const int rows = (int)min((int64_t)TILE_ROWS, n - i0), col0 = blockIdx.y * TILE_COLS, width = c.kv_heads * c.dh;
+    const T* src = is_v ? v + i0 * ldv + col0 : k + i0 * ldk + col0;
+    const int64_t ld = is_v ? ldv : ldk;
+#pragma unroll
+    for (int j = 0; j < TILE_ROWS * CHUNKS / 256; ++j) {
+        const int x = threadIdx.x + 256 * j, r = x / CHUNKS, e = (x % CHUNKS) * E;
+        if (r < rows && col0 + e < width)
+            *reinterpret_cast<uint4*>(tile + r * RowTile<T>::ROW_BYTES + e * (int)sizeof(T)) = *reinterpret_cast<const uint4*>(src + r * ld + e);
     }
+    __syncthreads();
+    const int groups = c.dh >> 5, hg = blockIdx.y * 4 + w;
+    if (hg >= c.kv_heads * groups) return;
+    const int64_t slot = lane < rows ? slots[i0 + lane] : -1;
+    const bool ok = slot >= 0 && slot < c.slots;
+    const unsigned char* mine = tile + (lane < rows ? lane : 0) * RowTile<T>::ROW_BYTES + w * 32 * (int)sizeof(T);
+    float x[32];
+#pragma unroll
+    for (int e = 0; e < 32; e += E) {
+        const uint4 u = *reinterpret_cast<const uint4*>(mine + e * (int)sizeof(T));
+        if (E == 4) {
+            x[e] = __uint_as_float(u.x); x[e + 1] = __uint_as_float(u.y); x[e + 2] = __uint_as_float(u.z); x[e + 3] = __uint_as_float(u.w);
+        } else {
+            x[e] = low_f(u.x); x[e + 1] = high_f(u.x); x[e + 2] = low_f(u.y); x[e + 3] = high_f(u.y);
+            x[e + E - 4] = low_f(u.z); x[e + E - 3] = high_f(u.z); x[e + E - 2] = low_f(u.w); x[e + E - 1] = high_f(u.w);
+        }
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
     const int s = scale_byte(top);
-    const float inv = inverse_scale(s == 255 ? 127 : s);
-    uint8_t* codes = blockIdx.z == 0 ? c.kc + (ph * page + tok) * (c.dh >> 1) + g * 16 : c.vc + (ph * (c.dh >> 1) + g * 16) * page + tok;
-    const int64_t step = blockIdx.z == 0 ? 1 : page;
-    for (int e = 0; e < 16; ++e) codes[e * step] = (uint8_t)(code_of(x[2 * e] * inv) | (code_of(x[2 * e + 1] * inv) << 4));
-    uint8_t* sc = blockIdx.z == 0 ? c.ks + (ph * page + tok) * groups + g : c.vs + (ph * groups + g) * page + tok;
-    *sc = (uint8_t)s;
+    const float unit = __uint_as_float(scale_to_bits(s == 255 ? 127 : s));
+    uint32_t codes[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {   // x * 2^-E, rounded to the nearest code, ties to the even one
+        codes[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[8 * d], x[8 * d + 1], unit, 0);
+        codes[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes[d], x[8 * d + 2], x[8 * d + 3], unit, 1);
+        codes[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes[d], x[8 * d + 4], x[8 * d + 5], unit, 2);
+        codes[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes[d], x[8 * d + 6], x[8 * d + 7], unit, 3);
+    }
+    const int h = hg / groups, g = hg - h * groups;
+    const int page = 1 << c.page_shift, tok = (int)slot & (page - 1);
+    const int64_t ph = (ok ? slot >> c.page_shift : 0) * c.kv_heads + h;
+    if (!is_v) {
+        if (!ok) return;
+        *reinterpret_cast<uint4*>(c.kc + ((ph << c.page_shift) + tok) * (c.dh >> 1) + g * 16) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+        c.ks[((ph << c.page_shift) + tok) * groups + g] = (uint8_t)s;
+        return;
+    }
+    uint8_t* vc = c.vc + ((ph * (c.dh >> 1) + g * 16) << c.page_shift);
+    if (ok) c.vs[((ph * groups + g) << c.page_shift) + tok] = (uint8_t)s;
+    // a quad whose slots are s, s + 1, s + 2, s + 3 of one page (a lane's slot is 32-bit)
+    const int q = lane & 3, s32 = ok ? (int)slot : -8;
+    const int first = __builtin_amdgcn_update_dpp(s32, s32, 0x00, 0xf, 0xf, false);      // the quad's lane 0
+    const bool fits = s32 == first + q && first >= 0 && (first & (page - 1)) + 3 < page;
+    const unsigned long long bal = __ballot(fits);
+    const bool quad = ((bal >> (lane & 60)) & 15ull) == 15ull;
+    const int tok0 = first & (page - 1);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const uint32_t t = quad_transpose(codes[d], q);                                  // every lane takes part in the exchange
+        if (quad) {
+            reinterpret_cast<word_any*>(vc + (((4 * d + q) << c.page_shift) + tok0))->v = t;
+        } else if (ok) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vc[((4 * d + e) << c.page_shift) + tok] = (uint8_t)(codes[d] >> (8 * e));
+        }
+    }
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void cache4_read_kernel(Cache c, const int32_t* __restrict__ slots, T* __restrict__ k, int64_t ldk,
                                                           T* __restrict__ v, int64_t ldv, int64_t n) {
-    const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int groups = c.dh >> 5;
-    const int hg = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (i >= n || hg >= c.kv_heads * groups) return;
-    const int64_t slot = slots[i];
-    const int h = hg / groups, g = hg - h * groups;
-    T* dst = (blockIdx.z == 0 ? k + i * ldk : v + i * ldv) + h * c.dh + g * 32;
-    if (slot < 0 || slot >= c.slots) {
-        for (int e = 0; e < 32; ++e) store1(dst + e, 0.0f);
-        return;
+    __shared__ __attribute__((aligned(16))) unsigned char tile[TILE_ROWS * RowTile<T>::ROW_BYTES];
+    constexpr int E = 16 / (int)sizeof(T), CHUNKS = RowTile<T>::CHUNKS;
+    const bool is_v = blockIdx.z != 0;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t i0 = (int64_t)blockIdx.x * TILE_ROWS;
+    const int rows = (int)min((int64_t)TILE_ROWS, n - i0), col0 = blockIdx.y * TILE_COLS, width = c.kv_heads * c.dh;
+    const int groups = c.dh >> 5, hg = blockIdx.y * 4 + w;
+    if (hg < c.kv_heads * groups) {
+        const int64_t slot = lane < rows ? slots[i0 + lane] : -1;
+        const bool ok = slot >= 0 && slot < c.slots;
+        const int h = hg / groups, g = hg - h * groups;
+        const int page = 1 << c.page_shift, tok = (int)slot & (page - 1);
+        const int64_t ph = (ok ? slot >> c.page_shift : 0) * c.kv_heads + h;
+        uint32_t codes[4] = {0u, 0u, 0u, 0u}, s = 127u;
+        if (ok) {
+            if (!is_v) {
+                const uint4 u = *reinterpret_cast<const uint4*>(c.kc + ((ph << c.page_shift) + tok) * (c.dh >> 1) + g * 16);
+                codes[0] = u.x; codes[1] = u.y; codes[2] = u.z; codes[3] = u.w;
+                s = c.ks[((ph << c.page_shift) + tok) * groups + g];
+            } else {
+                const uint8_t* vc = c.vc + ((ph * (c.dh >> 1) + g * 16) << c.page_shift) + tok;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) codes[e >> 2] |= (uint32_t)vc[e << c.page_shift] << (8 * (e & 3));
+                s = c.vs[((ph * groups + g) << c.page_shift) + tok];
+            }
+        }
+        unsigned char* mine = tile + lane * RowTile<T>::ROW_BYTES + w * 32 * (int)sizeof(T);
+        const uint32_t f = scale_to_bits((int)s);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            if (E == 8) {
+                *reinterpret_cast<uint4*>(mine + d * 16) = make_uint4(cvt4<0>(codes[d], f), cvt4<1>(codes[d], f), cvt4<2>(codes[d], f), cvt4<3>(codes[d], f));
+            } else {
+                const f32x2 a0 = cvt4f<0>(codes[d], f), a1 = cvt4f<1>(codes[d], f), a2 = cvt4f<2>(codes[d], f), a3 = cvt4f<3>(codes[d], f);
+                *reinterpret_cast<float4*>(mine + d * 32) = make_float4(a0[0], a0[1], a1[0], a1[1]);
+                *reinterpret_cast<float4*>(mine + d * 32 + 16) = make_float4(a2[0], a2[1], a3[0], a3[1]);
+            }
+        }
     }
-    const int page = 1 << c.page_shift;
-    const int64_t ph = (slot >> c.page_shift) * c.kv_heads + h;
-    const int tok = (int)(slot & (page - 1));
-    const uint8_t* codes = blockIdx.z == 0 ? c.kc + (ph * page + tok) * (c.dh >> 1) + g * 16 : c.vc + (ph * (c.dh >> 1) + g * 16) * page + tok;
-    const int64_t step = blockIdx.z == 0 ? 1 : page;
-    const float f = scale_of(blockIdx.z == 0 ? c.ks[(ph * page + tok) * groups + g] : c.vs[(ph * groups + g) * page + tok]);
-    for (int e = 0; e < 16; ++e) {
-        const uint32_t b = codes[e * step];
-        store1(dst + 2 * e, value_of(b & 15u) * f);
-        store1(dst + 2 * e + 1, value_of(b >> 4) * f);
+    __syncthreads();
+    T* dst = is_v ? v + i0 * ldv + col0 : k + i0 * ldk + col0;
+    const int64_t ld = is_v ? ldv : ldk;
+#pragma unroll
+    for (int j = 0; j < TILE_ROWS * CHUNKS / 256; ++j) {
+        const int x = threadIdx.x + 256 * j, r = x / CHUNKS, e = (x % CHUNKS) * E;
+        if (r < rows && col0 + e < width)
+            *reinterpret_cast<uint4*>(dst + r * ld + e) = *reinterpret_cast<const uint4*>(tile + r * RowTile<T>::ROW_BYTES + e * (int)sizeof(T));
     }
 }
 
@@ -122,22 +227,10 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Cache c, const int32_t
 // Long contexts are split over workgroups (rows x key heads x chunks) and, inside one, over its waves (tile by tile in turn); partial
 // (maximum, sum, O) are joined in LDS and by combine_kernel, in a fixed order.
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-
 union Frag {
     uint32_t u[4];
     bf16x8 v;
 };
-
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    const bf16x2 v = __builtin_convertvector(f32x2{a, b}, bf16x2);
-    return __builtin_bit_cast(uint32_t, v);
-}
-__device__ __forceinline__ float low_f(uint32_t u) { return __uint_as_float(u << 16); }
-__device__ __forceinline__ float high_f(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
 __device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpret_cast<f32x2*>(p) = f32x2{a, b}; }
 __device__ __forceinline__ void store2(__bf16* p, float a, float b) { *reinterpret_cast<uint32_t*>(p) = pack2(a, b); }
@@ -154,11 +247,6 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&p)[NP]) {
     }
 }
 
-// elements 2 SEL, 2 SEL + 1 of a word of codes; the conversion reads bits 23 .. 30 of the scale only
-template <int SEL>
-__device__ __forceinline__ uint32_t cvt4(uint32_t codes, uint32_t scale_bits) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, __uint_as_float(scale_bits), SEL));
-}
 // byte b of a word of scales, moved to bits 23 .. 30
 __device__ __forceinline__ uint32_t scale_bits(uint32_t w, int b) { return b == 0 ? w << 23 : (b == 1 ? w << 15 : (b == 2 ? w << 7 : w >> 1)); }
 
@@ -584,7 +672,7 @@ int cache4_write(const tst_cache4* c, const T* k, int64_t ldk, const T* v, int64
     int rc = check_cache(c, &d, who);
     if (rc == TST_OK) rc = check_rows(d, k, ldk, v, ldv, slots, n, who);
     if (rc != TST_OK || n == 0) return rc;
-    const dim3 grid((unsigned)((n + 63) / 64), (unsigned)((d.kv_heads * (d.dh >> 5) + 3) / 4), 2);
+    const dim3 grid((unsigned)((n + TILE_ROWS - 1) / TILE_ROWS), (unsigned)((d.kv_heads * d.dh + TILE_COLS - 1) / TILE_COLS), 2);
     cache4_write_kernel<T><<<grid, 256, 0, (hipStream_t)stream>>>(d, k, ldk, v, ldv, slots, n);
     return tst_after_launch(who);
 }
@@ -595,7 +683,7 @@ int cache4_read(const tst_cache4* c, const int32_t* slots, T* k, int64_t ldk, T*
     int rc = check_cache(c, &d, who);
     if (rc == TST_OK) rc = check_rows(d, k, ldk, v, ldv, slots, n, who);
     if (rc != TST_OK || n == 0) return rc;
-    const dim3 grid((unsigned)((n + 63) / 64), (unsigned)((d.kv_heads * (d.dh >> 5) + 3) / 4), 2);
+    const dim3 grid((unsigned)((n + TILE_ROWS - 1) / TILE_ROWS), (unsigned)((d.kv_heads * d.dh + TILE_COLS - 1) / TILE_COLS), 2);
     cache4_read_kernel<T><<<grid, 256, 0, (hipStream_t)stream>>>(d, slots, k, ldk, v, ldv, n);
     return tst_after_launch(who);
 }

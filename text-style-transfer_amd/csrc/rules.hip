@@ -3,59 +3,133 @@
 
 namespace {
 
-constexpr int CHUNK = 8192;              // columns per workgroup: one 32-bit counter each in LDS
 constexpr uint32_t SEEN = 0x80000000u;   // counter bit: the token is in the prompt
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const __bf16* p) { return (float)*p; }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(__bf16* p, float v) { *p = (__bf16)v; }
+__device__ __forceinline__ void load16(const float* p, float (&x)[4]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+__device__ __forceinline__ void load16(const __bf16* p, float (&x)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[2 * e] = __uint_as_float(u[e] << 16);
+        x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void store16(float* p, const float (&x)[4]) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
+__device__ __forceinline__ void store16(__bf16* p, const float (&x)[8]) {
+    bf16x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (__bf16)x[e];
+    *reinterpret_cast<bf16x8*>(p) = v;
+}
 
-// One workgroup per row and chunk of columns: the row's tokens are counted in LDS (integer atomics: the order does not matter),
-// then the chunk streams through once.
-template <typename T>
+// One workgroup per row and chunk of CHUNK columns: the row's tokens are counted in LDS, one 32-bit counter per column (integer atomics: the
+// order does not matter), then the chunk streams through once, 16 bytes per lane.  HBM-bound: the logits are read and written once, the
+// row's few hundred tokens are read once per chunk out of the caches.  Chunks begin where the row's addresses are 16-byte aligned, whatever
+// the row's own alignment (`shift` columns before that; a row is only handled element by element where logits and out differ in it).
+// In place (`out` is `logits`), pieces that no rule changes are neither read nor written.
+template <typename T, int CHUNK>
 __global__ __launch_bounds__(256) void adjust_logits_kernel(const T* logits, int64_t ld, int V, tst_logit_rules a, T* out, int64_t ldo) {
-    __shared__ uint32_t count[CHUNK];
+    __shared__ __attribute__((aligned(16))) uint32_t count[CHUNK];
+    constexpr int E = 16 / (int)sizeof(T);
     const int t = threadIdx.x;
     const int64_t r = blockIdx.y;
-    const int v0 = blockIdx.x * CHUNK, nv = min(CHUNK, V - v0);
+    const T* row_in = logits + r * ld;
+    T* row_out = out + r * ldo;
+    const int shift = (int)((reinterpret_cast<uintptr_t>(row_in) & 15u) / sizeof(T));
+    const bool vec = ((reinterpret_cast<uintptr_t>(row_in) ^ reinterpret_cast<uintptr_t>(row_out)) & 15u) == 0u;
+    const int v0 = (int)blockIdx.x * CHUNK - shift;                  // column of count[0]; below 0 in the first chunk of an unaligned row
+    if (v0 >= V) return;
     const int64_t s = a.sent != nullptr ? a.sent[r] : r;
-    const bool penal = a.params != nullptr && s >= 0 && s < a.n_sent;
+    int64_t p_lo = 0, p_hi = 0, n_hist = 0;
     float rp = 1.0f, fp = 0.0f, pp = 0.0f;
-    if (penal) {
+    if (a.params != nullptr && s >= 0 && s < a.n_sent) {
         rp = a.params[3 * s]; fp = a.params[3 * s + 1]; pp = a.params[3 * s + 2];
-        for (int i = t; i < nv; i += 256) count[i] = 0u;
-        __syncthreads();
         if (a.prompt != nullptr) {
-            const int64_t lo = max((int64_t)a.prompt_cu[s], (int64_t)0), hi = min((int64_t)a.prompt_cu[s + 1], a.n_prompt);
-            for (int64_t i = lo + t; i < hi; i += 256) {
-                const uint32_t c = (uint32_t)a.prompt[i] - (uint32_t)v0;
-                if (c < (uint32_t)nv) atomicOr(&count[c], SEEN);
-            }
+            p_lo = max((int64_t)a.prompt_cu[s], (int64_t)0);
+            p_hi = min((int64_t)a.prompt_cu[s + 1], a.n_prompt);
         }
-        if (a.hist != nullptr) {
-            const int64_t n = a.hist_len != nullptr ? min((int64_t)a.hist_len[r], a.n_hist) : a.n_hist;
-            for (int64_t i = t; i < n; i += 256) {
-                const uint32_t c = (uint32_t)a.hist[r * a.ld_hist + i] - (uint32_t)v0;
-                if (c < (uint32_t)nv) atomicAdd(&count[c], 1u);
-            }
+        if (a.hist != nullptr) n_hist = a.hist_len != nullptr ? min((int64_t)a.hist_len[r], a.n_hist) : a.n_hist;
+    }
+    const bool penal = p_hi > p_lo || n_hist > 0;
+    if (penal) {
+        for (int i = t; i < CHUNK / 4; i += 256) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+#pragma unroll 4
+        for (int64_t i = p_lo + t; i < p_hi; i += 256) {
+            const int v = a.prompt[i];
+            if (v >= max(v0, 0) && v < min(v0 + CHUNK, V)) atomicOr(&count[v - v0], SEEN);
+        }
+        const int32_t* hist = a.hist + r * a.ld_hist;
+#pragma unroll 4
+        for (int64_t i = t; i < n_hist; i += 256) {
+            const int v = hist[i];
+            if (v >= max(v0, 0) && v < min(v0 + CHUNK, V)) atomicAdd(&count[v - v0], 1u);
         }
         __syncthreads();
     }
     const int64_t br = a.bias == nullptr ? -1 : (a.bias_row != nullptr ? a.bias_row[r] : 0);
     const int64_t mr = a.mask == nullptr ? -1 : (a.mask_row != nullptr ? a.mask_row[r] : 0);
-    const float* bias = br >= 0 && br < a.n_bias ? a.bias + br * a.ld_bias + v0 : nullptr;
-    const uint32_t* mask = mr >= 0 && mr < a.n_masks ? a.mask + mr * a.ld_mask + (v0 >> 5) : nullptr;
-    for (int i = t; i < nv; i += 256) {
-        float y = load1(logits + r * ld + v0 + i);
-        if (penal) {
-            const uint32_t c = count[i];
-            if (c != 0u) y = y > 0.0f ? y / rp : y * rp;
+    const float* bias = br >= 0 && br < a.n_bias ? a.bias + br * a.ld_bias : nullptr;
+    const uint32_t* mask = mr >= 0 && mr < a.n_masks ? a.mask + mr * a.ld_mask : nullptr;
+    const int words = (V + 31) >> 5;
+    auto rules = [&](float y, int v, uint32_t c, bool allowed) {
+        if (c != 0u) {
+            y = y > 0.0f ? y / rp : y * rp;
             if ((c & ~SEEN) != 0u) y = (y - (float)(c & ~SEEN) * fp) - pp;
         }
-        if (bias != nullptr) y = y + bias[i];
-        if (mask != nullptr && ((mask[i >> 5] >> (i & 31)) & 1u) == 0u) y = -INFINITY;
-        store1(out + r * ldo + v0 + i, y);
+        if (bias != nullptr) y = y + bias[v];
+        return allowed ? y : -INFINITY;
+    };
+    for (int i = t; i < CHUNK / E; i += 256) {
+        const int c0 = v0 + i * E;                                   // columns c0 .. c0 + E - 1
+        if (c0 >= V) break;
+        if (vec && c0 >= 0 && c0 + E <= V) {
+            uint32_t n[E], any = 0u;
+#pragma unroll
+            for (int e = 0; e < E; ++e) n[e] = 0u;
+            if (penal) {
+#pragma unroll
+                for (int e = 0; e < E; e += 4) {
+                    const uint4 u = reinterpret_cast<const uint4*>(count)[(i * E + e) >> 2];
+                    n[e] = u.x; n[e + 1] = u.y; n[e + 2] = u.z; n[e + 3] = u.w;
+                    any |= u.x | u.y | u.z | u.w;
+                }
+            }
+            uint32_t allow = (1u << E) - 1u;
+            if (mask != nullptr) {
+                const int w = c0 >> 5;
+                uint64_t bits = mask[w];
+                if ((c0 & 31) + E > 32 && w + 1 < words) bits |= (uint64_t)mask[w + 1] << 32;
+                allow &= (uint32_t)(bits >> (c0 & 31));
+            }
+            if (out == logits && any == 0u && bias == nullptr && allow == (1u << E) - 1u) continue;
+            float x[E];
+            if (allow != 0u) {
+                load16(row_in + c0, x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = rules(x[e], c0 + e, n[e], (allow >> e) & 1u);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = -INFINITY;
+            }
+            store16(row_out + c0, x);
+        } else {
+            for (int e = 0; e < E; ++e) {
+                const int v = c0 + e;
+                if (v < 0 || v >= V) continue;
+                const bool allowed = mask == nullptr || ((mask[v >> 5] >> (v & 31)) & 1u) != 0u;
+                store1(row_out + v, rules(load1(row_in + v), v, penal ? count[v - v0] : 0u, allowed));
+            }
+        }
     }
 }
 
@@ -87,7 +161,10 @@ int adjust_logits(const T* logits, int64_t ld, int64_t R, int64_t V, const tst_l
     TST_REQUIRE(a->params == nullptr || a->sent != nullptr || a->n_sent >= R, TST_ERR_ARG, "%s: params must hold %lld rows", who, (long long)R);
     if (R == 0 || V == 0) return TST_OK;
     TST_REQUIRE(R <= 0x7fffffff / 4, TST_ERR_UNSUPPORTED, "%s: too many rows", who);
-    const int chunks = (int)((V + CHUNK - 1) / CHUNK);
+    // Long chunks read a row's tokens less often; few rows are cut finer, to have more workgroups than CUs
+    const bool fine = R * ((V + 8191) / 8192) < 512;
+    const int64_t chunk = fine ? 2048 : 8192;
+    const unsigned chunks = (unsigned)((V + 16 + chunk - 1) / chunk);       // a row may begin up to 7 columns into its first chunk
     for (int64_t r0 = 0; r0 < R; r0 += 65535) {   // grid.y holds at most 65535 rows
         const int64_t n = R - r0 < 65535 ? R - r0 : 65535;
         tst_logit_rules b = *a;
@@ -103,7 +180,9 @@ int adjust_logits(const T* logits, int64_t ld, int64_t R, int64_t V, const tst_l
                 b.n_sent -= r0;
             }
         }
-        adjust_logits_kernel<T><<<dim3((unsigned)chunks, (unsigned)n), 256, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
+        const dim3 grid(chunks, (unsigned)n);
+        if (fine) adjust_logits_kernel<T, 2048><<<grid, 256, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
+        else adjust_logits_kernel<T, 8192><<<grid, 256, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
         const int rc = tst_after_launch(who);
         if (rc != TST_OK) return rc;
     }
