@@ -6,6 +6,7 @@ namespace {
 constexpr uint32_t SEEN = 0x80000000u;   // counter bit: the token is in the prompt
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float float4_any __attribute__((ext_vector_type(4), aligned(4)));   // four floats at any float's address
 __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const __bf16* p) { return (float)*p; }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
@@ -31,14 +32,21 @@ __device__ __forceinline__ void store16(__bf16* p, const float (&x)[8]) {
     *reinterpret_cast<bf16x8*>(p) = v;
 }
 
-// One workgroup per row and chunk of CHUNK columns: the row's tokens are counted in LDS, one 32-bit counter per column (integer atomics: the
-// order does not matter), then the chunk streams through once, 16 bytes per lane.  HBM-bound: the logits are read and written once, the
-// row's few hundred tokens are read once per chunk out of the caches.  Chunks begin where the row's addresses are 16-byte aligned, whatever
-// the row's own alignment (`shift` columns before that; a row is only handled element by element where logits and out differ in it).
-// In place (`out` is `logits`), pieces that no rule changes are neither read nor written.
+// One workgroup per row and chunk of CHUNK columns, HBM-bound: the logits are read and written once, the row's tokens once per chunk out of
+// the caches.
+//   1. The row's tokens are counted in LDS, one 32-bit counter per column (integer atomics: the order does not matter); whoever finds
+//      a counter at 0 puts the column on a list.
+//   2. The listed columns' logits are penalised and left in place of their counters, as the complement of their bits (0 = no such
+//      token): a few divisions per row with all lanes at work, instead of a branch per column in the stream.
+//   3. The chunk streams through, 16 bytes per lane: penalised value or logit, bias, mask.
+// Chunks begin where the row's addresses are 16-byte aligned, whatever the row's own alignment (`shift` columns before it); a row is only
+// handled element by element where logits and out are aligned differently.  In place (`out` is `logits`), pieces that no rule changes
+// are neither read nor written.
 template <typename T, int CHUNK>
 __global__ __launch_bounds__(256) void adjust_logits_kernel(const T* logits, int64_t ld, int V, tst_logit_rules a, T* out, int64_t ldo) {
     __shared__ __attribute__((aligned(16))) uint32_t count[CHUNK];
+    __shared__ uint16_t list[CHUNK];
+    __shared__ int listed;
     constexpr int E = 16 / (int)sizeof(T);
     const int t = threadIdx.x;
     const int64_t r = blockIdx.y;
@@ -49,30 +57,50 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const T* logits, int
     const int v0 = (int)blockIdx.x * CHUNK - shift;                  // column of count[0]; below 0 in the first chunk of an unaligned row
     if (v0 >= V) return;
     const int64_t s = a.sent != nullptr ? a.sent[r] : r;
-    int64_t p_lo = 0, p_hi = 0, n_hist = 0;
+    int p_lo = 0, p_hi = 0, n_hist = 0;
     float rp = 1.0f, fp = 0.0f, pp = 0.0f;
     if (a.params != nullptr && s >= 0 && s < a.n_sent) {
         rp = a.params[3 * s]; fp = a.params[3 * s + 1]; pp = a.params[3 * s + 2];
         if (a.prompt != nullptr) {
-            p_lo = max((int64_t)a.prompt_cu[s], (int64_t)0);
-            p_hi = min((int64_t)a.prompt_cu[s + 1], a.n_prompt);
+            p_lo = max(a.prompt_cu[s], 0);
+            p_hi = min(a.prompt_cu[s + 1], (int)a.n_prompt);
         }
-        if (a.hist != nullptr) n_hist = a.hist_len != nullptr ? min((int64_t)a.hist_len[r], a.n_hist) : a.n_hist;
+        if (a.hist != nullptr) n_hist = a.hist_len != nullptr ? min(a.hist_len[r], (int)a.n_hist) : (int)a.n_hist;
     }
     const bool penal = p_hi > p_lo || n_hist > 0;
     if (penal) {
         for (int i = t; i < CHUNK / 4; i += 256) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (t == 0) listed = 0;
         __syncthreads();
-#pragma unroll 4
-        for (int64_t i = p_lo + t; i < p_hi; i += 256) {
-            const int v = a.prompt[i];
-            if (v >= max(v0, 0) && v < min(v0 + CHUNK, V)) atomicOr(&count[v - v0], SEEN);
+        const int lo = max(v0, 0), n = min(v0 + CHUNK, V) - lo;
+        auto note = [&](int v, bool prompt) {
+            if ((uint32_t)(v - lo) >= (uint32_t)n) return;
+            const uint32_t old = prompt ? atomicOr(&count[v - v0], SEEN) : atomicAdd(&count[v - v0], 1u);
+            if (old == 0u) list[atomicAdd(&listed, 1)] = (uint16_t)(v - v0);
+        };
+        for (int64_t at = (int64_t)p_lo + t; at < p_hi; at += 1024) {
+            int v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = at + 256 * u < p_hi ? a.prompt[at + 256 * u] : -1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) note(v[u], true);
         }
         const int32_t* hist = a.hist + r * a.ld_hist;
-#pragma unroll 4
-        for (int64_t i = t; i < n_hist; i += 256) {
-            const int v = hist[i];
-            if (v >= max(v0, 0) && v < min(v0 + CHUNK, V)) atomicAdd(&count[v - v0], 1u);
+        for (int64_t at = t; at < n_hist; at += 1024) {
+            int v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = at + 256 * u < n_hist ? hist[at + 256 * u] : -1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) note(v[u], false);
+        }
+        __syncthreads();
+        for (int i = t; i < listed; i += 256) {
+            const int at = list[i];
+            const uint32_t c = count[at];
+            float y = load1(row_in + v0 + at);
+            y = y > 0.0f ? y / rp : y * rp;
+            if ((c & ~SEEN) != 0u) y = (y - (float)(c & ~SEEN) * fp) - pp;
+            count[at] = ~__float_as_uint(y);
         }
         __syncthreads();
     }
@@ -81,21 +109,11 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const T* logits, int
     const float* bias = br >= 0 && br < a.n_bias ? a.bias + br * a.ld_bias : nullptr;
     const uint32_t* mask = mr >= 0 && mr < a.n_masks ? a.mask + mr * a.ld_mask : nullptr;
     const int words = (V + 31) >> 5;
-    auto rules = [&](float y, int v, uint32_t c, bool allowed) {
-        if (c != 0u) {
-            y = y > 0.0f ? y / rp : y * rp;
-            if ((c & ~SEEN) != 0u) y = (y - (float)(c & ~SEEN) * fp) - pp;
-        }
-        if (bias != nullptr) y = y + bias[v];
-        return allowed ? y : -INFINITY;
-    };
     for (int i = t; i < CHUNK / E; i += 256) {
         const int c0 = v0 + i * E;                                   // columns c0 .. c0 + E - 1
         if (c0 >= V) break;
         if (vec && c0 >= 0 && c0 + E <= V) {
             uint32_t n[E], any = 0u;
-#pragma unroll
-            for (int e = 0; e < E; ++e) n[e] = 0u;
             if (penal) {
 #pragma unroll
                 for (int e = 0; e < E; e += 4) {
@@ -113,21 +131,32 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const T* logits, int
             }
             if (out == logits && any == 0u && bias == nullptr && allow == (1u << E) - 1u) continue;
             float x[E];
-            if (allow != 0u) {
-                load16(row_in + c0, x);
+            load16(row_in + c0, x);
+            if (any != 0u) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = rules(x[e], c0 + e, n[e], (allow >> e) & 1u);
-            } else {
+                for (int e = 0; e < E; ++e) x[e] = n[e] != 0u ? __uint_as_float(~n[e]) : x[e];
+            }
+            if (bias != nullptr) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = -INFINITY;
+                for (int e = 0; e < E; e += 4) {
+                    const float4_any b = *reinterpret_cast<const float4_any*>(bias + c0 + e);
+                    x[e] += b[0]; x[e + 1] += b[1]; x[e + 2] += b[2]; x[e + 3] += b[3];
+                }
+            }
+            if (allow != (1u << E) - 1u) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = ((allow >> e) & 1u) != 0u ? x[e] : -INFINITY;
             }
             store16(row_out + c0, x);
         } else {
             for (int e = 0; e < E; ++e) {
                 const int v = c0 + e;
                 if (v < 0 || v >= V) continue;
-                const bool allowed = mask == nullptr || ((mask[v >> 5] >> (v & 31)) & 1u) != 0u;
-                store1(row_out + v, rules(load1(row_in + v), v, penal ? count[v - v0] : 0u, allowed));
+                float y = load1(row_in + v);
+                if (penal && count[v - v0] != 0u) y = __uint_as_float(~count[v - v0]);
+                if (bias != nullptr) y = y + bias[v];
+                if (mask != nullptr && ((mask[v >> 5] >> (v & 31)) & 1u) == 0u) y = -INFINITY;
+                store1(row_out + v, y);
             }
         }
     }
@@ -162,8 +191,8 @@ int adjust_logits(const T* logits, int64_t ld, int64_t R, int64_t V, const tst_l
     if (R == 0 || V == 0) return TST_OK;
     TST_REQUIRE(R <= 0x7fffffff / 4, TST_ERR_UNSUPPORTED, "%s: too many rows", who);
     // Long chunks read a row's tokens less often; few rows are cut finer, to have more workgroups than CUs
-    const bool fine = R * ((V + 8191) / 8192) < 512;
-    const int64_t chunk = fine ? 2048 : 8192;
+    const bool fine = R * ((V + 4095) / 4096) < 512;
+    const int64_t chunk = fine ? 1024 : 4096;
     const unsigned chunks = (unsigned)((V + 16 + chunk - 1) / chunk);       // a row may begin up to 7 columns into its first chunk
     for (int64_t r0 = 0; r0 < R; r0 += 65535) {   // grid.y holds at most 65535 rows
         const int64_t n = R - r0 < 65535 ? R - r0 : 65535;
@@ -181,8 +210,8 @@ int adjust_logits(const T* logits, int64_t ld, int64_t R, int64_t V, const tst_l
             }
         }
         const dim3 grid(chunks, (unsigned)n);
-        if (fine) adjust_logits_kernel<T, 2048><<<grid, 256, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
-        else adjust_logits_kernel<T, 8192><<<grid, 256, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
+        if (fine) adjust_logits_kernel<T, 1024><<<grid, 256, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
+        else adjust_logits_kernel<T, 4096><<<grid, 256, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
         const int rc = tst_after_launch(who);
         if (rc != TST_OK) return rc;
     }
