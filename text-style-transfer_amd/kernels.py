@@ -630,48 +630,52 @@ def retire_compact(cur, nxt, sel, lp, n_sent, k, step, T, eos, last_step, top_en
 
 # ---- prompted decoding: packed prompts, pages, a cache in 4 bits, rules on logits --------------------------------------------------
 
-def _rows2d(t, dtype, n_rows, n_cols, name):
-    """A 2-D view on the current GPU whose rows the kernels can read 16 bytes at a time."""
-    unit = 16 // t.element_size()
-    if not (t.is_cuda and t.dtype == dtype and t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1)):
-        raise ValueError('%s must be a 2-D %s GPU tensor with unit inner stride' % (name, dtype))
-    if t.shape[0] < n_rows or t.shape[1] < n_cols:
-        raise ValueError('%s must hold [%d, %d], got %s' % (name, n_rows, n_cols, tuple(t.shape)))
-    if n_rows > 1 and (t.stride(0) < n_cols or t.stride(0) % unit):
+_I32, _U8, _F32, _BF16 = torch.int32, torch.uint8, torch.float32, torch.bfloat16
+_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)
+
+
+# The checks below run on every call of kernels that take a few microseconds: each asks a tensor for as little as it can.  All tensors
+# have to live on the current device, on whose current stream the kernels run (``dev``: its number; a CPU tensor answers -1).
+
+def _rows2d(t, dtype, dev, n_rows, n_cols, name):
+    """Leading dimension of a 2-D view whose rows the kernels can read 16 bytes at a time."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not dtype or len(shape) != 2 or t.get_device() != dev or (stride[1] != 1 and shape[1] > 1):
+        raise ValueError('%s must be a 2-D %s tensor with unit inner stride on the current GPU, got %s %s on %s'
+                         % (name, dtype, t.dtype, tuple(shape), t.device))
+    if shape[0] < n_rows or shape[1] < n_cols:
+        raise ValueError('%s must hold [%d, %d], got %s' % (name, n_rows, n_cols, tuple(shape)))
+    unit = 4 if dtype is _F32 else 8
+    ld = stride[0]
+    if n_rows <= 1:
+        ld = max(ld, n_cols)
+        ld += -ld % unit
+    elif ld < n_cols or ld % unit:
         raise ValueError('rows of %s must not overlap and start at multiples of %d elements (16 bytes)' % (name, unit))
     if t.data_ptr() % 16:
         raise ValueError('%s must start at a 16-byte boundary' % name)
+    return ld
 
 
-def _ld(t, n_cols, unit):
-    """Leading dimension of a view (of a single row any multiple of the unit that holds it will do)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), n_cols) // unit * unit + (unit if max(t.stride(0), n_cols) % unit else 0)
-
-
-def _ints(t, shape, name):
+def _ints(t, n, dev, name):
+    """Address of a 1-D int32 tensor of at least n entries (None: a null pointer)."""
     if t is None:
-        return
-    if not (t.is_cuda and t.dtype == torch.int32 and t.is_contiguous() and t.dim() == len(shape)
-            and all(a >= b for a, b in zip(t.shape, shape))):
-        raise ValueError('%s must be a contiguous int32 tensor %s on the GPU, got %s %s' % (name, list(shape), t.dtype, tuple(t.shape)))
+        return None
+    if t.dtype is not _I32 or t.dim() != 1 or t.numel() < n or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError('%s must be a contiguous int32 tensor [%d] on the current GPU, got %s %s on %s' % (name, n, t.dtype, tuple(t.shape), t.device))
+    return t.data_ptr()
 
 
-def _one_device(*tensors):
-    """The kernels run on the current device's stream: every tensor has to live there."""
-    dev = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != dev:
-            raise ValueError('a tensor is on %s, the current device is cuda:%d' % (t.device, dev))
+def _table(t, dev, name):
+    shape = t.shape
+    if t.dtype is not _I32 or len(shape) != 2 or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError('%s must be a contiguous 2-D int32 tensor on the current GPU, got %s %s on %s' % (name, t.dtype, tuple(shape), t.device))
+    return shape
 
 
-def _span(t, n_rows, n_cols):
-    """First and last byte of the first n_rows x n_cols of a 2-D view."""
-    lo = t.data_ptr()
-    return (lo, lo) if n_rows == 0 or n_cols == 0 else (lo, lo + ((n_rows - 1) * t.stride(0) + n_cols) * t.element_size())
-
-
-def _disjoint(a, b, what):
-    if a[0] < b[1] and b[0] < a[1]:
+def _disjoint(a, lda, b, ldb, n_rows, cols_a, cols_b, size, what):
+    """Raises if the first n_rows rows of two views (addresses, leading dimensions, widths, element size) share a byte's range."""
+    if n_rows > 0 and a < b + ((n_rows - 1) * ldb + cols_b) * size and b < a + ((n_rows - 1) * lda + cols_a) * size:
         raise ValueError(what)
 
 
@@ -679,26 +683,26 @@ def attn_prompt(q, k, v, cu, out, heads, kv_heads=None, scale=None):
     """Causal attention over packed prompts: rows cu[b] .. cu[b + 1] - 1 of q [N, heads * dh], k, v [N, kv_heads * dh] (views with
     unit inner stride, fp32 or bf16) are sequence b; head h reads key head h // (heads / kv_heads).  ``out`` [N, heads * dh] must not
     overlap them; its rows outside every sequence are left alone.  ``scale``: 1 / sqrt(dh) unless given."""
-    kv_heads = heads if kv_heads is None else kv_heads
-    if q.dtype not in (torch.float32, torch.bfloat16):
+    if kv_heads is None:
+        kv_heads = heads
+    dt, dev = q.dtype, _device()
+    if dt is not _BF16 and dt is not _F32:
         raise ValueError('q must be fp32 or bf16')
     if q.dim() != 2 or heads < 1 or kv_heads < 1 or heads % kv_heads or q.shape[1] % heads:
         raise ValueError('q must be [tokens, heads * head size], heads a multiple of kv_heads')
-    N, dh = q.shape[0], q.shape[1] // heads
-    unit = 16 // q.element_size()
+    N, wq = q.shape
+    dh = wq // heads
+    unit, size = (8, 2) if dt is _BF16 else (4, 4)
     if dh % unit or not 0 < dh <= 256:
         raise ValueError('head size %d is not a multiple of %d up to 256' % (dh, unit))
-    if cu.dim() != 1 or cu.numel() < 1:
-        raise ValueError('cu must be [sequences + 1]')
-    _ints(cu, (1,), 'cu')
-    for t, nm, w in ((q, 'q', heads * dh), (k, 'k', kv_heads * dh), (v, 'v', kv_heads * dh), (out, 'out', heads * dh)):
-        _rows2d(t, q.dtype, N, w, nm)
-    _one_device(q, k, v, cu, out)
-    for t, w in ((q, heads * dh), (k, kv_heads * dh), (v, kv_heads * dh)):
-        _disjoint(_span(out, N, heads * dh), _span(t, N, w), 'out must not overlap q, k or v')
-    call('tst_attn_prompt_bf16' if q.dtype == torch.bfloat16 else 'tst_attn_prompt_f32', _p(q), _ld(q, heads * dh, unit), _p(k),
-         _ld(k, kv_heads * dh, unit), _p(v), _ld(v, kv_heads * dh, unit), _p(cu), cu.numel() - 1, _p(out), _ld(out, heads * dh, unit), N, heads,
-         kv_heads, dh, float(dh ** -0.5 if scale is None else scale), _stream())
+    wk = kv_heads * dh
+    ldq, ldk = _rows2d(q, dt, dev, N, wq, 'q'), _rows2d(k, dt, dev, N, wk, 'k')
+    ldv, ldo = _rows2d(v, dt, dev, N, wk, 'v'), _rows2d(out, dt, dev, N, wq, 'out')
+    pq, pk, pv, po, pc = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ints(cu, 1, dev, 'cu')
+    for p, ld, w in ((pq, ldq, wq), (pk, ldk, wk), (pv, ldv, wk)):
+        _disjoint(po, ldo, p, ld, N, wq, w, size, 'out must not overlap q, k or v')
+    call('tst_attn_prompt_bf16' if dt is _BF16 else 'tst_attn_prompt_f32', pq, ldq, pk, ldk, pv, ldv, pc, cu.numel() - 1, po, ldo, N, heads, kv_heads,
+         dh, dh ** -0.5 if scale is None else scale, _stream())
 
 
 def page_plan(lens, room, pages, page, table, cu, slots, pos, seq, used):
@@ -706,32 +710,25 @@ def page_plan(lens, room, pages, page, table, cu, slots, pos, seq, used):
     ``pages`` in order.  Writes ``table`` [B, width] (-1 where there is no page), ``cu`` [B + 1], and per packed token ``slots``,
     ``pos``, ``seq`` (entries behind the last token stay as they are); ``used`` [1] = pages needed, more than ``pages`` holds if
     the list is too short (the entries that got none are -1).  All int32; ``page`` a power of two in 8 .. 1024."""
-    B = lens.numel()
-    _ints(lens, (B,), 'lens'); _ints(room, (B,), 'room'); _ints(pages, (0,), 'pages'); _ints(cu, (B + 1,), 'cu'); _ints(used, (1,), 'used')
-    if table.dim() != 2 or table.shape[0] != B:
+    dev = _device()
+    B, N, n_pages = lens.numel(), slots.numel(), pages.numel()
+    rows, width = _table(table, dev, 'table')
+    if rows != B:
         raise ValueError('table must be [sequences, width]')
-    _ints(table, (B, 0), 'table')
-    N = slots.numel()
-    for t, nm in ((slots, 'slots'), (pos, 'pos'), (seq, 'seq')):
-        _ints(t, (N,), nm)
-    _one_device(lens, room, pages, table, cu, slots, pos, seq, used)
-    if pages.numel() * page > 0x7fffffff:
+    if n_pages * page > 0x7fffffff:
         raise ValueError('pages * page exceeds 2^31 - 1: slots are 32-bit')
-    call('tst_page_plan', _p(lens), _p(room), B, _p(pages), pages.numel(), int(page), _p(table), table.shape[1], _p(cu), _p(slots), _p(pos),
-         _p(seq), N, _p(used), _stream())
+    call('tst_page_plan', _ints(lens, B, dev, 'lens'), _ints(room, B, dev, 'room'), B, _ints(pages, 0, dev, 'pages'), n_pages, page, table.data_ptr(),
+         width, _ints(cu, B + 1, dev, 'cu'), _ints(slots, N, dev, 'slots'), _ints(pos, N, dev, 'pos'), _ints(seq, N, dev, 'seq'), N,
+         _ints(used, 1, dev, 'used'), _stream())
 
 
 def page_step(base, sent, t, table, page, slots, pos, lens, n_rows):
     """Step ``t`` of decoding over a page table: row r continues sequence ``sent[r]`` (None: r) at position base + t: ``pos``, ``lens``
     (= pos + 1) and ``slots`` (-1 without a page) of the first ``n_rows`` rows."""
-    if table.dim() != 2:
-        raise ValueError('table must be [sequences, width]')
-    _ints(table, (0, 0), 'table'); _ints(base, (table.shape[0],), 'base'); _ints(sent, (n_rows,), 'sent')
-    for x, nm in ((slots, 'slots'), (pos, 'pos'), (lens, 'lens')):
-        _ints(x, (n_rows,), nm)
-    _one_device(base, sent, table, slots, pos, lens)
-    call('tst_page_step', _p(base), _p(sent), int(t), _p(table), table.shape[1], table.shape[0], int(page), _p(slots), _p(pos), _p(lens), n_rows,
-         _stream())
+    dev = _device()
+    n_seq, width = _table(table, dev, 'table')
+    call('tst_page_step', _ints(base, n_seq, dev, 'base'), _ints(sent, n_rows, dev, 'sent'), t, table.data_ptr(), width, n_seq, page,
+         _ints(slots, n_rows, dev, 'slots'), _ints(pos, n_rows, dev, 'pos'), _ints(lens, n_rows, dev, 'lens'), n_rows, _stream())
 
 
 class Cache4:
@@ -744,47 +741,50 @@ class Cache4:
             raise ValueError('head size %d is not 32, 64, 128 or 256' % head_size)
         if page not in (16, 32, 64, 128):
             raise ValueError('a page holds 16, 32, 64 or 128 tokens, not %d' % page)
-        if pages < 0 or kv_heads < 1 or pages * page > 0x7fffffff:
-            raise ValueError('pages * page must be below 2^31 (slots are 32-bit), kv_heads at least 1')
+        if pages < 0 or not 1 <= kv_heads <= 4096 or pages * page > 0x7fffffff:
+            raise ValueError('pages * page must be below 2^31 (slots are 32-bit), kv_heads in 1 .. 4096')
         self.pages, self.page, self.kv_heads, self.dh = pages, page, kv_heads, head_size
         shapes = ((pages, kv_heads, page, head_size // 2), (pages, kv_heads, page, head_size // 32),
                   (pages, kv_heads, head_size // 2, page), (pages, kv_heads, head_size // 32, page))
         if tensors is None:
             tensors = [torch.zeros(s, dtype=torch.uint8, device=device) for s in shapes]
         for t, s, nm in zip(tensors, shapes, ('kc', 'ks', 'vc', 'vs')):
-            if not (t.is_cuda and t.dtype == torch.uint8 and tuple(t.shape) == s and t.is_contiguous() and t.data_ptr() % 16 == 0):
+            if not (t.is_cuda and t.device == tensors[0].device and t.dtype is _U8 and tuple(t.shape) == s and t.is_contiguous()
+                    and t.data_ptr() % 16 == 0):
                 raise ValueError('%s must be a contiguous, 16-byte aligned uint8 tensor %s on the GPU' % (nm, list(s)))
         self.kc, self.ks, self.vc, self.vs = tensors
+        self.dev = tensors[0].get_device()
         self.c = _lib.TstCache4(kc=_p(self.kc), ks=_p(self.ks), vc=_p(self.vc), vs=_p(self.vs), pages=pages, page=page, kv_heads=kv_heads,
                                 dh=head_size, reserved=0)
 
-
-def _cache_rows(cache, k, v, slots, n_rows):
-    w = cache.kv_heads * cache.dh
-    if k.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError('rows must be fp32 or bf16')
-    _rows2d(k, k.dtype, n_rows, w, 'k'); _rows2d(v, k.dtype, n_rows, w, 'v'); _ints(slots, (n_rows,), 'slots')
-    _one_device(cache.kc, k, v, slots)
-    unit = 16 // k.element_size()
-    return _ld(k, w, unit), _ld(v, w, unit), '_bf16' if k.dtype == torch.bfloat16 else '_f32'
+    def _on(self, dev):
+        if self.dev != dev:
+            raise ValueError('the cache is on cuda:%d, the current device is cuda:%d' % (self.dev, dev))
+        return self.c
 
 
 def cache4_write(cache, k, v, slots, n_rows):
     """Rows 0 .. n_rows - 1 of k and v ([n, kv_heads * dh], fp32 or bf16) into the cache at ``slots`` (page * page size + token; a
     slot outside the cache stores nothing; no slot twice)."""
-    ldk, ldv, ty = _cache_rows(cache, k, v, slots, n_rows)
-    call('tst_cache4_write' + ty, cache.c, _p(k), ldk, _p(v), ldv, _p(slots), n_rows, _stream())
+    dt, w, dev = k.dtype, cache.kv_heads * cache.dh, _device()
+    if dt is not _BF16 and dt is not _F32:
+        raise ValueError('rows must be fp32 or bf16')
+    call('tst_cache4_write_bf16' if dt is _BF16 else 'tst_cache4_write_f32', cache._on(dev), k.data_ptr(), _rows2d(k, dt, dev, n_rows, w, 'k'), v.data_ptr(),
+         _rows2d(v, dt, dev, n_rows, w, 'v'), _ints(slots, n_rows, dev, 'slots'), n_rows, _stream())
 
 
 def cache4_read(cache, slots, k, v, n_rows):
-    """The rows at ``slots`` as the values their codes stand for (zeros for a slot outside the cache)."""
-    ldk, ldv, ty = _cache_rows(cache, k, v, slots, n_rows)
-    call('tst_cache4_read' + ty, cache.c, _p(slots), _p(k), ldk, _p(v), ldv, n_rows, _stream())
+    """The rows at ``slots`` as the values their codes stand for (zeros for a slot outside the cache); k and v must not overlap."""
+    dt, w, dev = k.dtype, cache.kv_heads * cache.dh, _device()
+    if dt is not _BF16 and dt is not _F32:
+        raise ValueError('rows must be fp32 or bf16')
+    call('tst_cache4_read_bf16' if dt is _BF16 else 'tst_cache4_read_f32', cache._on(dev), _ints(slots, n_rows, dev, 'slots'), k.data_ptr(),
+         _rows2d(k, dt, dev, n_rows, w, 'k'), v.data_ptr(), _rows2d(v, dt, dev, n_rows, w, 'v'), n_rows, _stream())
 
 
 def attn_cache4_work(n_rows, heads, kv_heads, head_size, max_len, device='cuda'):
-    """The scratch tensor ``attn_cache4`` wants for calls of up to these sizes, or None where it needs none.  Calls that may run at
-    the same time (streams, captured graphs) need one each."""
+    """The scratch tensor ``attn_cache4`` wants for calls of these sizes, or None where it needs none.  Calls that may run at the same
+    time (streams, captured graphs) need one each."""
     n = _lib._dll.tst_attn_cache4_work(n_rows, heads, kv_heads, head_size, max_len)
     if n < 0:
         raise ValueError('bad sizes')
@@ -795,25 +795,32 @@ def attn_cache4(q, cache, table, lens, out, n_rows, heads, max_len, seq=None, sc
     """One step's attention over a 4-bit cache: row r of q [n_rows, heads * dh] (fp32 or bf16) attends to the first ``lens[r]`` tokens
     of sequence ``seq[r]`` (None: r) of the page table.  No token to attend to gives zeros.  ``max_len``: an upper bound of
     ``lens`` (longer rows are cut to it).  ``work``: scratch of ``attn_cache4_work``, made here when None."""
-    w = heads * cache.dh
-    if q.dtype not in (torch.float32, torch.bfloat16):
+    dt, dh, dev = q.dtype, cache.dh, _device()
+    if dt is not _BF16 and dt is not _F32:
         raise ValueError('q must be fp32 or bf16')
     if heads < 1 or heads % cache.kv_heads:
-        raise ValueError('heads must be a multiple of the cache\'s %d' % cache.kv_heads)
-    _rows2d(q, q.dtype, n_rows, w, 'q'); _rows2d(out, q.dtype, n_rows, w, 'out')
-    if table.dim() != 2:
-        raise ValueError('table must be [sequences, width]')
-    _ints(table, (0, 0), 'table'); _ints(lens, (n_rows,), 'lens'); _ints(seq, (n_rows,), 'seq')
+        raise ValueError("heads must be a multiple of the cache's %d" % cache.kv_heads)
+    w = heads * dh
+    ldq, ldo = _rows2d(q, dt, dev, n_rows, w, 'q'), _rows2d(out, dt, dev, n_rows, w, 'out')
+    pq, po = q.data_ptr(), out.data_ptr()
+    _disjoint(po, ldo, pq, ldq, n_rows, w, w, 2 if dt is _BF16 else 4, 'out must not overlap q')
+    n_seq, width = _table(table, dev, 'table')
     if work is None:
-        work = attn_cache4_work(n_rows, heads, cache.kv_heads, cache.dh, max_len, q.device)
-    elif not (work.is_cuda and work.dtype == torch.float32 and work.is_contiguous()):
-        raise ValueError('work must be a contiguous fp32 GPU tensor')
-    _one_device(q, cache.kc, table, lens, out, seq, work)
-    _disjoint(_span(out, n_rows, w), _span(q, n_rows, w), 'out must not overlap q')
-    unit = 16 // q.element_size()
-    call('tst_attn_cache4_bf16' if q.dtype == torch.bfloat16 else 'tst_attn_cache4_f32', cache.c, _p(q), _ld(q, w, unit), _p(table), table.shape[1],
-         table.shape[0], _p(seq), _p(lens), int(max_len), _p(out), _ld(out, w, unit), n_rows, heads,
-         float(cache.dh ** -0.5 if scale is None else scale), _p(work), 0 if work is None else work.numel(), _stream())
+        work = attn_cache4_work(n_rows, heads, cache.kv_heads, dh, max_len, q.device)
+    elif work.dtype is not _F32 or work.get_device() != dev or not work.is_contiguous():
+        raise ValueError('work must be a contiguous fp32 tensor on the current GPU')
+    call('tst_attn_cache4_bf16' if dt is _BF16 else 'tst_attn_cache4_f32', cache._on(dev), pq, ldq, table.data_ptr(), width, n_seq,
+         _ints(seq, n_rows, dev, 'seq'), _ints(lens, n_rows, dev, 'lens'), max_len, po, ldo, n_rows, heads, dh ** -0.5 if scale is None else scale,
+         None if work is None else work.data_ptr(), 0 if work is None else work.numel(), _stream())
+
+
+def _rule_rows(t, dtype, width, dev, name):
+    """(address, leading dimension, rows) of a bias or mask table."""
+    shape, stride = t.shape, t.stride()
+    if (t.dtype is not dtype or len(shape) != 2 or t.get_device() != dev or shape[1] < width or (stride[1] != 1 and shape[1] > 1)
+            or (shape[0] > 1 and stride[0] < width)):
+        raise ValueError('%s must be a 2-D %s tensor [n, %d] with unit inner stride on the current GPU' % (name, dtype, width))
+    return t.data_ptr(), max(stride[0], width), shape[0]
 
 
 def adjust_logits(logits, n_rows, n_cols, out, *, params=None, sent=None, hist=None, hist_len=None, prompt=None, prompt_cu=None, bias=None,
@@ -823,55 +830,60 @@ def adjust_logits(logits, n_rows, n_cols, out, *, params=None, sent=None, hist=N
     or per row), ``bias`` [n, >= V] fp32, ``mask`` [n, >= ceil(V / 32)] int32 words (bit 0 = forbidden = -inf).  ``hist`` [rows, n]
     int32 tokens with ``hist_len`` [rows] valid ones (None: all); ``prompt`` packed int32 tokens with offsets ``prompt_cu`` [n + 1];
     ``bias_row`` / ``mask_row`` [rows] choose a row (None: row 0, -1: none).  ``out`` may be ``logits``.  fp32 or bf16."""
-    suffix = _logits_suffix(logits)
-    if logits.dim() != 2 or out.dim() != 2 or out.dtype != logits.dtype or not out.is_cuda or out.stride(1) != 1:
-        raise ValueError('logits and out must be 2-D GPU tensors of one type with unit inner stride')
-    if min(logits.shape[0], out.shape[0]) < n_rows or min(logits.shape[1], out.shape[1]) < n_cols:
-        raise ValueError('logits and out must hold [%d, %d]' % (n_rows, n_cols))
-    if n_rows > 1 and min(logits.stride(0), out.stride(0)) < n_cols:
-        raise ValueError('rows must not overlap')
-    if logits.data_ptr() != out.data_ptr():
-        _disjoint(_span(logits, n_rows, n_cols), _span(out, n_rows, n_cols), 'out must be logits or not overlap it')
-    n_sent = 0
+    dev, dt = _device(), logits.dtype
+    if dt is not _F32 and dt is not _BF16:
+        raise ValueError('logits must be fp32 or bf16')
+    lds = []
+    for t, nm in ((logits, 'logits'), (out, 'out')):
+        shape, stride = t.shape, t.stride()
+        if t.dtype is not dt or len(shape) != 2 or t.get_device() != dev or (stride[1] != 1 and shape[1] > 1):
+            raise ValueError('logits and out must be 2-D tensors of one type with unit inner stride on the current GPU')
+        if shape[0] < n_rows or shape[1] < n_cols or (n_rows > 1 and stride[0] < n_cols):
+            raise ValueError('%s must hold [%d, %d] without overlapping rows' % (nm, n_rows, n_cols))
+        lds.append(max(stride[0], n_cols))
+    p_in, p_out = logits.data_ptr(), out.data_ptr()
+    if p_in != p_out:
+        _disjoint(p_out, lds[1], p_in, lds[0], n_rows, n_cols, n_cols, 4 if dt is _F32 else 2, 'out must be logits or not overlap it')
+    rules = _lib.TstLogitRules()
     if params is not None:
-        _chk(params, torch.float32, 'params')
-        if params.dim() != 2 or params.shape[1] != 3 or (sent is None and params.shape[0] < n_rows):
-            raise ValueError('params must be [sentences, 3]')
-        n_sent = params.shape[0]
+        if (params.dtype is not _F32 or params.dim() != 2 or params.shape[1] != 3 or params.get_device() != dev or not params.is_contiguous()
+                or (sent is None and params.shape[0] < n_rows)):
+            raise ValueError('params must be a contiguous fp32 tensor [sentences, 3] on the current GPU')
+        rules.params, rules.n_sent = params.data_ptr(), params.shape[0]
     elif hist is not None or prompt is not None:
         raise ValueError('hist and prompt need params')
-    _ints(sent, (n_rows,), 'sent'); _ints(hist_len, (n_rows,), 'hist_len'); _ints(prompt, (0,), 'prompt')
-    if hist is not None and not (hist.is_cuda and hist.dtype == torch.int32 and hist.dim() == 2 and hist.shape[0] >= n_rows
-                                 and (hist.stride(1) == 1 or hist.shape[1] <= 1) and (n_rows <= 1 or hist.stride(0) >= hist.shape[1])):
-        raise ValueError('hist must be int32 [rows, tokens] on the GPU with unit inner stride')
+    if sent is not None:
+        rules.sent = _ints(sent, n_rows, dev, 'sent')
+    if hist is not None:
+        shape, stride = hist.shape, hist.stride()
+        if (hist.dtype is not _I32 or len(shape) != 2 or hist.get_device() != dev or shape[0] < n_rows or (stride[1] != 1 and shape[1] > 1)
+                or (n_rows > 1 and stride[0] < shape[1])):
+            raise ValueError('hist must be int32 [rows, tokens] with unit inner stride on the current GPU')
+        rules.hist, rules.ld_hist, rules.n_hist = hist.data_ptr(), max(stride[0], shape[1]), shape[1]
+        rules.hist_len = _ints(hist_len, n_rows, dev, 'hist_len')
     if prompt is not None:
         if prompt_cu is None:
             raise ValueError('prompt needs prompt_cu')
-        _ints(prompt_cu, (n_sent + 1,), 'prompt_cu')
-    for t, rows, nm, dt, width in ((bias, bias_row, 'bias', torch.float32, n_cols), (mask, mask_row, 'mask', torch.int32, (n_cols + 31) // 32)):
-        _ints(rows, (n_rows,), nm + '_row')
-        if t is not None and not (t.is_cuda and t.dtype == dt and t.dim() == 2 and t.shape[1] >= width
-                                  and (t.stride(1) == 1 or t.shape[1] <= 1) and (t.shape[0] <= 1 or t.stride(0) >= width)):
-            raise ValueError('%s must be a %s GPU tensor [n, %d] with unit inner stride' % (nm, dt, width))
-    _one_device(logits, out, params, sent, hist, hist_len, prompt, prompt_cu, bias, bias_row, mask, mask_row)
-    ld = lambda t, w: 0 if t is None else max(t.stride(0), w)     # noqa: E731
-    rules = _lib.TstLogitRules(
-        params=_p(params), sent=_p(sent), n_sent=n_sent, hist=_p(hist), ld_hist=0 if hist is None else max(hist.stride(0), hist.shape[1]),
-        n_hist=0 if hist is None else hist.shape[1], hist_len=_p(hist_len), prompt=_p(prompt), n_prompt=0 if prompt is None else prompt.numel(),
-        prompt_cu=_p(prompt_cu), bias=_p(bias), ld_bias=ld(bias, n_cols), n_bias=0 if bias is None else bias.shape[0], bias_row=_p(bias_row),
-        mask=_p(mask), ld_mask=ld(mask, (n_cols + 31) // 32), n_masks=0 if mask is None else mask.shape[0], mask_row=_p(mask_row))
-    call('tst_adjust_logits' + suffix, _p(logits), max(logits.stride(0), n_cols), n_rows, n_cols, rules, _p(out), max(out.stride(0), n_cols), _stream())
+        rules.prompt, rules.n_prompt = _ints(prompt, 0, dev, 'prompt'), prompt.numel()
+        rules.prompt_cu = _ints(prompt_cu, rules.n_sent + 1, dev, 'prompt_cu')
+    if bias is not None:
+        rules.bias, rules.ld_bias, rules.n_bias = _rule_rows(bias, _F32, n_cols, dev, 'bias')
+        rules.bias_row = _ints(bias_row, n_rows, dev, 'bias_row')
+    if mask is not None:
+        rules.mask, rules.ld_mask, rules.n_masks = _rule_rows(mask, _I32, (n_cols + 31) // 32, dev, 'mask')
+        rules.mask_row = _ints(mask_row, n_rows, dev, 'mask_row')
+    call('tst_adjust_logits_bf16' if dt is _BF16 else 'tst_adjust_logits_f32', p_in, lds[0], n_rows, n_cols, rules, p_out, lds[1], _stream())
 
 
 def grammar_next(table, state, parent, tok, out, n_rows):
     """out[r] = table[state[parent[r]], tok[r]] (``parent`` None: r); -1 stays -1 and is what leaves the table."""
-    if table.dim() != 2:
-        raise ValueError('table must be [states, V]')
-    _ints(table, (0, 0), 'table'); _ints(state, (0,), 'state'); _ints(parent, (n_rows,), 'parent'); _ints(tok, (n_rows,), 'tok'); _ints(out, (n_rows,), 'out')
-    _one_device(table, state, parent, tok, out)
-    if out.data_ptr() == state.data_ptr():
+    dev = _device()
+    n_states, V = _table(table, dev, 'table')
+    ps, po = _ints(state, 0, dev, 'state'), _ints(out, n_rows, dev, 'out')
+    if po == ps:
         raise ValueError('out must not be state')
-    call('tst_grammar_next', _p(table), table.shape[0], table.shape[1], _p(state), state.numel(), _p(parent), _p(tok), _p(out), n_rows, _stream())
+    call('tst_grammar_next', table.data_ptr(), n_states, V, ps, state.numel(), _ints(parent, n_rows, dev, 'parent'), _ints(tok, n_rows, dev, 'tok'), po, n_rows,
+         _stream())
 
 
 class PagedPlan:
