@@ -7,6 +7,7 @@ requires the built library (``csrc/build.sh``); there is no CPU or PyTorch fallb
 from . import _lib
 from ._lib import TstError, version
 from .vocab import Vocab
+from .engine import Grammar
 from .inference import InferenceState, simple_inference
 from .transformer import HP, Transformer, TransformerDecoder
 from .encoder import TransformerEncoder
@@ -17,4 +18,4 @@ from .streams import run_on_streams
 
 __all__ = ['InferenceState', 'simple_inference', 'Vocab', 'HP', 'Transformer', 'TransformerDecoder', 'TransformerEncoder',
            'RNNDecoder', 'RNNEncoder', 'Generator', 'FFN', 'RNNLM', 'ConditionalLM', 'WeightedLMEnsemble', 'CharLMFromEmbs',
-           'TransformerLM', 'itos_many', 'compute_bleu_for_sents', 'corpus_bleu', 'run_on_streams', 'TstError', 'version']
+           'TransformerLM', 'itos_many', 'compute_bleu_for_sents', 'corpus_bleu', 'run_on_streams', 'Grammar', 'TstError', 'version']

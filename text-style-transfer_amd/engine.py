@@ -73,9 +73,120 @@ def _pinned_counts(dev):
     return _PINNED[key]
 
 
+def _per_sentence(x, n_sent, name, lo=None):
+    """A number or one number per sentence as fp32 [n_sent] on the host."""
+    t = torch.as_tensor(x, dtype=torch.float32).detach().cpu()
+    t = t.expand(n_sent) if t.dim() == 0 else t
+    if tuple(t.shape) != (n_sent,) or not bool(torch.isfinite(t).all()) or (lo is not None and not bool((t > lo).all())):
+        raise ValueError('%s must be a finite number%s or one per sentence' % (name, '' if lo is None else ' above %g' % lo))
+    return t
+
+
+def pack_mask(allowed):
+    """Boolean [n, V] as the bit rows [n, ceil(V / 32)] int32 that the rule kernels read (bit v % 32 of word v / 32)."""
+    n, V = allowed.shape
+    bits = torch.zeros((n, (V + 31) // 32 * 32), dtype=torch.int64, device=allowed.device)
+    bits[:, :V] = allowed
+    words = (bits.view(n, -1, 32) << torch.arange(32, device=allowed.device)).sum(-1)
+    return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)     # the same bits as a signed word
+
+
+class Grammar:
+    """A finite automaton over tokens: ``next[s, v]`` (int [states, V]) is the state after token v in state s, -1 where v is
+    forbidden; decoding starts in state ``start`` (a number, or one per sentence).  Every state must allow some token."""
+
+    def __init__(self, next, start=0):
+        t = torch.as_tensor(next)
+        if t.dim() != 2 or t.is_floating_point() or t.shape[0] < 1 or t.shape[1] < 1:
+            raise ValueError('next must be integers [states, V]')
+        if int(t.min()) < -1 or int(t.max()) >= t.shape[0]:
+            raise ValueError('next holds states outside -1 .. %d' % (t.shape[0] - 1))
+        if not bool((t >= 0).any(1).all()):
+            raise ValueError('state %d allows no token' % int((t < 0).all(1).nonzero()[0]))
+        self.next, self.start = t.to(torch.int32), start
+
+    def on(self, device, n_sent, V):
+        """(table, bit masks, start states) on the device"""
+        if self.next.shape[1] != V:
+            raise ValueError('the grammar has %d tokens, the vocabulary %d' % (self.next.shape[1], V))
+        start = torch.as_tensor(self.start, dtype=torch.int32).cpu()
+        start = start.expand(n_sent) if start.dim() == 0 else start
+        if tuple(start.shape) != (n_sent,) or int(start.min()) < 0 or int(start.max()) >= self.next.shape[0]:
+            raise ValueError('start must be a state, or one per sentence')
+        table = self.next.to(device).contiguous()
+        return table, pack_mask(table >= 0), start.to(device)
+
+
+class LogitRules:
+    """What a decode call does to the logits before it picks tokens: penalties for repeated tokens, biases, token masks, a grammar.
+    ``prompts``: token ids of every sentence before the first step (they count for the repetition penalty only).  The state per row is the
+    loop's own token history, and the grammar state of each row, which ``advance`` carries through selection, retirement and beam
+    reorders."""
+
+    def __init__(self, V, n_sent, beam, device, repetition_penalty=1.0, frequency_penalty=0.0, presence_penalty=0.0, logit_bias=None,
+                 allowed_tokens=None, grammar=None, prompts=None):
+        self.V = V
+        self.params = self.prompt = self.prompt_cu = self.bias = self.mask = self.table = self.state = None
+        self.bias_by_sent = self.mask_by_sent = False
+        rep = _per_sentence(repetition_penalty, n_sent, 'repetition_penalty', 0.0)
+        freq = _per_sentence(frequency_penalty, n_sent, 'frequency_penalty')
+        pres = _per_sentence(presence_penalty, n_sent, 'presence_penalty')
+        if bool((rep != 1).any()) or bool((freq != 0).any()) or bool((pres != 0).any()):
+            self.params = torch.stack((rep, freq, pres), 1).contiguous().to(device)
+            if prompts is not None and bool((rep != 1).any()):
+                lens = torch.tensor([0] + [len(p) for p in prompts], dtype=torch.int64)
+                self.prompt_cu = lens.cumsum(0).to(torch.int32).to(device)
+                self.prompt = torch.cat([torch.as_tensor(p).reshape(-1).to(device=device, dtype=torch.int32) for p in prompts])
+        if logit_bias is not None:
+            if isinstance(logit_bias, dict):
+                ids = torch.tensor(list(logit_bias), dtype=torch.int64)
+                if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= V):
+                    raise IndexError('logit_bias names token ids outside the vocabulary (0..%d)' % (V - 1))
+                b = torch.zeros(V)
+                b[ids] = torch.tensor([float(x) for x in logit_bias.values()], dtype=torch.float32)
+            else:
+                b = torch.as_tensor(logit_bias)
+            if tuple(b.shape) not in ((V,), (n_sent, V)) or bool(torch.isnan(b.float()).any()) or bool((b.float() == float('inf')).any()):
+                raise ValueError('logit_bias must be a dict {token id: bias} or a tensor [V] or [batch, V] without NaN and +inf')
+            self.bias_by_sent = b.dim() == 2
+            self.bias = b.reshape(-1, V).to(device=device, dtype=torch.float32).contiguous()
+        if allowed_tokens is not None and grammar is not None:
+            raise ValueError('a grammar says which tokens are allowed: allowed_tokens cannot be given as well')
+        if allowed_tokens is not None:
+            ok = torch.as_tensor(allowed_tokens)
+            if tuple(ok.shape) not in ((V,), (n_sent, V)) or ok.dtype != torch.bool:
+                raise ValueError('allowed_tokens must be a boolean tensor [V] or [batch, V]')
+            if not bool(ok.reshape(-1, V).any(1).all()):
+                raise ValueError('allowed_tokens leaves a sentence no token')
+            self.mask_by_sent = ok.dim() == 2
+            self.mask = pack_mask(ok.reshape(-1, V).to(device))
+        if grammar is not None:
+            self.table, self.mask, start = grammar.on(device, n_sent, V)
+            rows = n_sent * beam
+            self.state, self.spare = (torch.full((rows,), -1, dtype=torch.int32, device=device) for _ in range(2))
+            self.state[:n_sent] = start
+
+    @property
+    def active(self):
+        return self.params is not None or self.bias is not None or self.mask is not None
+
+    def apply(self, logits, out, rows, n_rows, first, n_generated):
+        """``out`` = the logits of ``n_rows`` rows after the rules; the row's generated tokens are hist[first : first + n_generated]."""
+        hist = rows.hist[:, first:first + n_generated] if self.params is not None and n_generated > 0 else None
+        K.adjust_logits(logits, n_rows, self.V, out, params=self.params, sent=rows.sent if self.params is not None else None, hist=hist,
+                        prompt=self.prompt, prompt_cu=self.prompt_cu, bias=self.bias, bias_row=rows.sent if self.bias_by_sent else None,
+                        mask=self.mask, mask_row=self.state if self.state is not None else (rows.sent if self.mask_by_sent else None))
+
+    def advance(self, row_parent, tok, n_rows):
+        """After a step: row r continues row ``row_parent[r]`` with token ``tok[r]``."""
+        if self.state is not None:
+            K.grammar_next(self.table, self.state, row_parent, tok, self.spare, n_rows)
+            self.state, self.spare = self.spare, self.state
+
+
 class DecodeLoop:
     def __init__(self, session, n_sent, beam, max_len, bos, eos, pad, alpha=0.0, device=None, sample=None, gumbel=None,
-                 prefix=None):
+                 prefix=None, rules=None):
         if not (1 <= beam <= 8):
             raise ValueError('beam_size must be in 1..8')
         if beam > session.V:
@@ -131,7 +242,10 @@ class DecodeLoop:
             self.lse = torch.zeros(R, dtype=torch.float32, device=dev)
         self.tail = None   # kernels.SelectPlan, made at the first step (it needs the session's logits buffer)
         self.keys = None   # arg-max keys of greedy steps (see _keys_for)
-        if (KEYS_ON and beam == 1 and sample is None and gumbel is None and getattr(session, 'keys_ok', None) is not None):
+        self.rules = rules if rules is not None and rules.active else None     # LogitRules, applied to every step's logits
+        self.adjusted = None                                                   # where they go when the logits are not the session's own
+        if (KEYS_ON and beam == 1 and sample is None and gumbel is None and self.rules is None
+                and getattr(session, 'keys_ok', None) is not None):
             self.keys = torch.zeros((R, K.ARGMAX_SLOTS), dtype=torch.int64, device=dev)
         # Soft decoding (``gumbel=True`` of /root/reference/src/inference.py:104-105,136-138): the next input of a row
         # is the distribution softmax((softmax(logits) + G) / temperature) instead of a token id; the token that
@@ -161,6 +275,19 @@ class DecodeLoop:
             return None
         return self.keys
 
+    def _apply_rules(self, logits, R, t):
+        """The step's logits after the rules: in place where the buffer is the session's own, else in a buffer of the loop (a foreign
+        model may hand out memory that it goes on using)."""
+        _check_logits(logits, R, self.s.V)
+        out = logits
+        if not getattr(self.s, 'incremental', False):
+            if self.adjusted is None or self.adjusted.dtype != logits.dtype or self.adjusted.shape[0] < R:
+                self.adjusted = torch.empty((R if self.adjusted is None else max(R, self.adjusted.shape[0]), (self.s.V + 7) // 8 * 8),
+                                            dtype=logits.dtype, device=self.dev)
+            out = self.adjusted
+        self.rules.apply(logits, out, self.cur, R, self.pos0 + 1, t)
+        return out
+
     def run(self, keep_logits=0):
         """Runs the loop.  Returns (out_tok [B, pos0 + T + 1], out_len [B], out_score [B]) on the device; with
         ``keep_logits`` > 0 also records (logits, sentence ids of the rows) of the first steps in
@@ -189,6 +316,8 @@ class DecodeLoop:
                 logits = s.step(self.cur, R, t, soft=self.dist_in)
             if t < keep_logits:
                 self.kept.append((logits[:R, :s.V].clone(), self.cur.sent[:R].clone(), self.cur.fin[:R].clone()))
+            if self.rules is not None:
+                logits = self._apply_rules(logits, R, t)
             if self.gumbel is None and self.select_log is None:
                 # selection, retirement and compaction: one native call
                 if self.tail is None:
@@ -197,7 +326,7 @@ class DecodeLoop:
                                              top_idx=self.top_idx, lse=self.lse, sel=self.sel, lp=self.lp, T=Ttot,
                                              top_ends=self.top_ends, sample=self.sample, out_tok=self.out_tok, out_len=self.out_len,
                                              out_score=self.out_score, scratch=self.scratch, row_parent=self.row_parent,
-                                             n_alive=self.n_alive, stats=getattr(s, 'stats', None))
+                                             n_alive=self.n_alive, stats=getattr(s, 'stats', None) if self.rules is None else None)
                 elif logits.data_ptr() != self.tail.logits_ptr:
                     _check_logits(logits, R, s.V)
                     self.tail.set_logits(logits)
@@ -228,6 +357,8 @@ class DecodeLoop:
             if alive == 0:
                 break
             s.reorder(self.row_parent, alive * k, identity=(k == 1 and alive == n_sent))
+            if self.rules is not None:
+                self.rules.advance(self.row_parent, self.cur.tok, alive * k)
             if self.gumbel is not None:
                 K.gather_rows(self.dist_out, self.row_parent, self.dist_in, alive)
             n_sent = alive
@@ -251,13 +382,15 @@ class DecodeLoop:
             logits = s.step(self.cur, R, pos0 + t) if keys is None else s.step(self.cur, R, pos0 + t, keys=keys)
             if t < keep_logits:
                 self.kept.append((logits[:R, :s.V].clone(), self.cur.sent[:R].clone(), self.cur.fin[:R].clone()))
+            if self.rules is not None:
+                logits = self._apply_rules(logits, R, t)
             if self.tail is None:
                 _check_logits(logits, R, s.V)
                 self.tail = K.SelectPlan(k=k, eos=self.eos, V=s.V, logits=logits, am=self.am, top_val=self.top_val,
                                          top_idx=self.top_idx, lse=self.lse, sel=self.sel, lp=self.lp, T=Ttot,
                                          top_ends=self.top_ends, sample=self.sample, out_tok=self.out_tok, out_len=self.out_len,
                                          out_score=self.out_score, scratch=self.scratch, row_parent=self.row_parent,
-                                         n_alive=self.n_alive, stats=getattr(s, 'stats', None))
+                                         n_alive=self.n_alive, stats=getattr(s, 'stats', None) if self.rules is None else None)
             elif logits.data_ptr() != self.tail.logits_ptr:
                 _check_logits(logits, R, s.V)
                 self.tail.set_logits(logits)
@@ -272,6 +405,8 @@ class DecodeLoop:
             self.cur, self.nxt = self.nxt, self.cur
             self.steps_done += 1
             self.rows_stepped += R
+            if self.rules is not None:
+                self.rules.advance(self.row_parent, self.cur.tok, bound * k)
             if t == 0:                                  # every sentence entered step 0: the bound is exact
                 s.reorder(self.row_parent, bound * k, identity=False)
                 continue

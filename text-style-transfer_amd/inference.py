@@ -16,6 +16,16 @@ so ``torch.manual_seed`` governs it like it governs the reference's ``Categorica
 CPU generator exactly as ``/root/reference/src/utils/gumbel.py:12`` does and copies them to the GPU, so the same
 ``torch.manual_seed`` gives the reference's noise; ``'device'`` draws them on the GPU).
 
+``kv_cache``: ``'fp4'`` decodes a ``TransformerLM`` over a cache held in 4 bits (greedy or sampling, not beams): about a fifth of the
+bf16 cache's bytes, prompts run through the model at once instead of token by token, and ``active_seqs`` may then also be a list of
+B prompts (1-D id tensors) of different lengths.  Rounding keys and values to 4 bits changes logits; the default keeps them whole.
+
+``repetition_penalty`` (> 0; divides positive and multiplies negative logits of tokens that the prompt or the output holds),
+``frequency_penalty`` (times a token's count in the output, subtracted), ``presence_penalty`` (subtracted once) — each a number or one
+per sentence —, ``logit_bias`` (dict {id: bias}, or a tensor [V] or [B, V]), ``allowed_tokens`` (boolean [V] or [B, V]) and ``grammar``
+(an ``engine.Grammar``): rules applied to the logits of every step, in this order, before the token selection.  They work with every
+model, with beams (a hypothesis follows its own history and grammar state) and with sampling.
+
 ``active_seqs`` (``:37``): a caller-provided prefix of token ids ``[B, t0]`` replaces the single BOS; results start with
 it and may grow to ``t0 + max_len`` tokens (the loop still runs ``max_len`` steps, ``:155``).
 
@@ -33,7 +43,7 @@ per step exactly as the reference does, on GPU tensors, and only the selection /
 """
 import torch
 
-from .engine import DecodeLoop
+from .engine import DecodeLoop, LogitRules
 
 
 class ForeignSession:
@@ -126,6 +136,10 @@ class InferenceState:
         self.return_logits = state_dict.get('return_logits', False)
         self.step_logits = []
 
+        self.kv_cache = state_dict.get('kv_cache')
+        self.rules = {k: state_dict[k] for k in ('repetition_penalty', 'frequency_penalty', 'presence_penalty', 'logit_bias',
+                                                 'allowed_tokens', 'grammar') if state_dict.get(k) is not None}
+
         self.finished = [None for _ in range(self.batch_size)]
         self.num_steps_done = 0
         self.validate()
@@ -138,6 +152,16 @@ class InferenceState:
         # bos/eos must be in the dictionary (/root/reference/src/inference.py:56-58)
         assert self.bos_idx != self.vocab.stoi[self.unk_token]
         assert self.eos_idx != self.vocab.stoi[self.unk_token]
+
+    def _prompts(self, prefix):
+        """The tokens of every sentence before the first step, one 1-D tensor each."""
+        if prefix is None:
+            return [torch.tensor([self.bos_idx])] * self.batch_size
+        return list(prefix)
+
+    def _check_ids(self, ids):
+        if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= len(self.vocab)):   # nn.Embedding raises IndexError there
+            raise IndexError('active_seqs holds token ids outside the vocabulary (0..%d)' % (len(self.vocab) - 1))
 
     def _session(self, n_positions=None):
         if hasattr(self.model, 'session') and not self.kwargs.get('force_foreign', False):
@@ -171,13 +195,27 @@ class InferenceState:
                     raise ValueError("sample_type='sample' needs beam_size 1")
                 seed = self.seed if self.seed is not None else int(torch.randint(0, 2 ** 31 - 1, (1,)).item())
                 sample = (float(self.temperature), seed)
+            if self.kv_cache not in (None, 'fp4'):
+                raise ValueError("kv_cache must be None or 'fp4'")
             prefix = None
-            if self.active_seqs is not None and not self.gumbel:
+            if self.kv_cache is not None:
+                if not hasattr(self.model, 'paged_session') or self.kwargs.get('force_foreign', False):
+                    raise NotImplementedError("kv_cache='fp4' is supported for TransformerLM")
+                if self.beam_size != 1 or self.gumbel:
+                    raise NotImplementedError("kv_cache='fp4' decodes one token sequence per sentence: no beams, no gumbel")
+            if isinstance(self.active_seqs, (list, tuple)):
+                if self.kv_cache is None:
+                    raise NotImplementedError("prompts of different lengths (active_seqs as a list) need kv_cache='fp4'")
+                prefix = [torch.as_tensor(p) for p in self.active_seqs]
+                if len(prefix) != self.batch_size or any(p.dim() != 1 or p.numel() < 1 or p.is_floating_point() for p in prefix):
+                    raise ValueError('active_seqs must be one 1-D tensor of at least one token id per sentence')
+                for p in prefix:
+                    self._check_ids(p)
+            elif self.active_seqs is not None and not self.gumbel:
                 prefix = self.active_seqs
                 if prefix.dim() != 2 or prefix.shape[0] != self.batch_size or prefix.shape[1] < 1 or prefix.is_floating_point():
                     raise ValueError('active_seqs must be token ids [batch, t0 >= 1]')
-                if int(prefix.min()) < 0 or int(prefix.max()) >= len(self.vocab):   # nn.Embedding raises IndexError there
-                    raise IndexError('active_seqs holds token ids outside the vocabulary (0..%d)' % (len(self.vocab) - 1))
+                self._check_ids(prefix)
             if not torch.cuda.is_available():
                 raise RuntimeError('InferenceState needs a GPU: the decode loop runs in HIP kernels and has no CPU path')
             device = self.inputs.device if self.inputs.is_cuda else torch.device('cuda', torch.cuda.current_device())
@@ -204,8 +242,17 @@ class InferenceState:
                     draw = lambda n, v: torch.rand((n, v), device=device)        # noqa: E731
                 gumbel = (float(self.temperature), dist_prefix, draw)
             with torch.cuda.device(device):
-                total = self.max_len if prefix is None else self.max_len + prefix.shape[1] - 1
-                session = self._session(total)
+                rules = None
+                if self.rules:
+                    rules = LogitRules(len(self.vocab), self.batch_size, self.beam_size, device, prompts=self._prompts(prefix), **self.rules)
+                self.prompts = None
+                if self.kv_cache is not None:
+                    # the session runs the prompts; the loop starts from their last tokens
+                    self.prompts = [p.to(device=device, dtype=torch.long) for p in self._prompts(prefix)]
+                    session = self.model.paged_session(self.inputs, self.prompts, self.max_len)
+                    prefix = torch.stack([p[-1] for p in self.prompts]).unsqueeze(1)
+                else:
+                    session = self._session(self.max_len if prefix is None else self.max_len + prefix.shape[1] - 1)
                 if prefix is not None and prefix.shape[1] > 1:
                     if isinstance(session, ForeignSession):
                         session.pos0 = prefix.shape[1] - 1
@@ -216,7 +263,7 @@ class InferenceState:
                         raise NotImplementedError('an id prefix longer than one token together with substitute_inputs is only '
                                                   'supported for foreign model callables')
                 loop = DecodeLoop(session, self.batch_size, self.beam_size, self.max_len, self.bos_idx,
-                                  self.eos_idx, self.pad_idx, self.length_penalty, device, sample, gumbel, prefix)
+                                  self.eos_idx, self.pad_idx, self.length_penalty, device, sample, gumbel, prefix, rules)
                 loop.select_log = getattr(self, 'select_log', None)
                 loop.run(keep_logits)
         finally:
@@ -231,7 +278,7 @@ class InferenceState:
     def decode_packed(self):
         """Runs the loop and returns the outputs as device tensors, without building the reference's list of
         per-sentence tensors: (tokens [B, 1 + max_len] int32, padded with ``<pad>``; lengths [B] int32, BOS
-        included and EOS stripped; scores [B] fp32)."""
+        included and EOS stripped; scores [B] fp32).  With ``kv_cache`` the tokens start at the last one of every prompt."""
         loop = self._run()
         return loop.out_tok, loop.out_len, loop.out_score
 
@@ -248,6 +295,8 @@ class InferenceState:
             return self.finished
         toks = loop.out_tok.long()
         self.finished = [toks[i, :n] for i, n in enumerate(lens)]
+        if self.prompts is not None:
+            self.finished = [torch.cat((p[:-1], s)) for p, s in zip(self.prompts, self.finished)]
         if self.should_stack_finished:
             self.stack_finished()
         return self.finished

@@ -116,6 +116,31 @@ class TransformerLM(HipModule):
     def session(self, z, enc_mask=None, rows_per_sentence=1, max_len=None):
         return TransformerLMSession(self, z, rows_per_sentence, max_len if max_len is not None else self.pe_max_len)
 
+    def paged_session(self, z, prompts, max_new, page=32):
+        """Decode state over ragged prompts: a 4-bit paged cache that holds all but the last token of every prompt (see ``PagedLMSession``)."""
+        return PagedLMSession(self, z, prompts, max_new, page)
+
+    def prompt_logits(self, z, seqs):
+        """z [B, model_size], seqs = B sequences of token ids (1-D, of any lengths) -> per sequence its raw logits [length, V] fp32: every
+        position attends to its prefix.  All sequences go through the model at once, packed (``kernels.attn_prompt``); ``lm(z, x)``
+        evaluates the same position by position in the step kernels' own summation order."""
+        z, toks, lens = _prompt_inputs(self, z, seqs, 0, 0)
+        n = sum(lens)
+        V = self.V
+        out = torch.empty((n, V), dtype=torch.float32, device=self.device)
+        if n > 0:
+            with torch.cuda.device(self.device if self.device.index is not None else torch.cuda.current_device()):
+                cu, pos, seq = _packed_index(lens, self.device)
+                h = _run_packed(self, z, toks, pos, seq, cu, n, None)
+                W = self.prepared()
+                if self.dtype == 'bf16':
+                    low = torch.empty((n, (V + 7) // 8 * 8), dtype=torch.bfloat16, device=self.device)
+                    K.gemm_bf16(h, W['wout'], W['bout'], low, n, n_cols=V)
+                    out.copy_(low[:, :V])
+                else:
+                    K.gemm(h, W['wout'], W['bout'], out, n)
+        return list(out.split(lens)) if lens else []
+
     # ---- reference call protocol: whole-prefix logits ------------------------------------------------
     def __call__(self, z, x):
         """z [B, model_size], x [B, t] ids -> raw logits [B, t, V] (every position attends to its prefix);
@@ -247,4 +272,125 @@ class TransformerLMSession:
             log.begin()
             plan.run(rows, n, t, K.STEP_VOCAB)
             log.end(2.0 * n * lm.d * self.V)
+        return self.logits
+
+
+def _prompt_inputs(lm, z, prompts, least, room):
+    """Checked inputs of a packed pass: (z fp32 [B, d], packed int32 tokens, lengths)."""
+    dev = lm.device
+    z = z.to(device=dev, dtype=torch.float32).contiguous()
+    if z.dim() != 2 or z.shape[1] != lm.d:
+        raise ValueError('z must be [B, model_size=%d], got %s' % (lm.d, tuple(z.shape)))
+    rows = [torch.as_tensor(p) for p in prompts]
+    if len(rows) != z.shape[0]:
+        raise ValueError('%d prompts for %d conditioning vectors' % (len(rows), z.shape[0]))
+    for p in rows:
+        if p.dim() != 1 or p.is_floating_point() or p.dtype == torch.bool or p.numel() < least:
+            raise ValueError('a prompt must be a 1-D tensor of at least %d token ids' % least)
+    lens = [int(p.numel()) for p in rows]
+    if lens and max(lens) + room > lm.pe_max_len:
+        raise ValueError('%d positions exceed pe_max_len %d' % (max(lens) + room, lm.pe_max_len))
+    toks = torch.cat([p.to(device=dev, dtype=torch.int64) for p in rows]) if rows else torch.empty(0, dtype=torch.int64, device=dev)
+    if toks.numel() and (int(toks.min()) < 0 or int(toks.max()) >= lm.V):       # nn.Embedding raises IndexError there
+        raise IndexError('a prompt holds token ids outside the vocabulary (0..%d)' % (lm.V - 1))
+    return z, toks.to(torch.int32), lens
+
+
+def _packed_index(lens, device):
+    """(offsets [B + 1], position and sequence of every packed token), int32"""
+    n = torch.tensor(lens, dtype=torch.int32, device=device)
+    B, total = len(lens), sum(lens)
+    i32 = dict(dtype=torch.int32, device=device)
+    cu, used = torch.empty(B + 1, **i32), torch.empty(1, **i32)
+    slots, pos, seq = (torch.empty(total, **i32) for _ in range(3))
+    K.page_plan(n, None, torch.empty(0, **i32), 32, torch.empty((B, 0), **i32), cu, slots, pos, seq, used)
+    return cu, pos, seq
+
+
+def _run_packed(lm, z, tok, pos, seq, cu, n, store):
+    """The layer stack over n packed tokens (sequences back to back, offsets ``cu``); ``store(layer, k, v)`` sees every layer's keys and
+    values.  Returns the final LayerNorm's output [n, d] in the model's activation type."""
+    W, dev, d = lm.prepared(), lm.device, lm.d
+    bf = lm.dtype == 'bf16'
+    lo = dict(dtype=torch.bfloat16 if bf else torch.float32, device=dev)
+    x = torch.empty((n, d), dtype=torch.float32, device=dev)
+    h, a = torch.empty((n, d), **lo), torch.empty((n, d), **lo)
+    qkv, ff = torch.empty((n, 3 * d), **lo), torch.empty((n, lm.d_ff), **lo)
+    gemm = K.gemm_bf16 if bf else K.gemm
+    K.embed_posadd_rows(tok, W['emb'], W['pe'], float(torch.tensor(math.sqrt(d), dtype=torch.float32)), z, seq, x, n, pos=pos)
+    for li, L in enumerate(W['layers']):
+        K.layernorm(x, L['ln1'][0], L['ln1'][1], h, n)
+        gemm(h, L['wqkv'], L['bqkv'], qkv, n)
+        q, k, v = qkv[:, :d], qkv[:, d:2 * d], qkv[:, 2 * d:]
+        if store is not None:
+            store(li, k, v)
+            if li == len(W['layers']) - 1:
+                return None                       # a prefill: nothing reads what the last layer would add
+        K.attn_prompt(q, k, v, cu, a, lm.heads)
+        gemm(a, L['wo'], L['bo'], x, n, res=x)
+        K.layernorm(x, L['ln2'][0], L['ln2'][1], h, n)
+        gemm(h, L['w1'], L['b1'], ff, n, act=1)
+        gemm(ff, L['w2'], L['b2'], x, n, res=x)
+    K.layernorm(x, W['ln'][0], W['ln'][1], h, n)
+    return h
+
+
+class PagedLMSession:
+    """Per-batch decode state of a ``TransformerLM`` over prompts of different lengths: every layer's keys and values live in a 4-bit
+    cache in pages (``kernels.Cache4``), mapped by a page table built on the GPU.  Making the session runs all but the last token of
+    every prompt through the model at once; ``step`` then takes one token per row, the last prompt token first, each row at its own
+    position.  One row per sentence (no beams); a row's pages belong to its sentence, so compaction moves nothing."""
+    needs_anc = False
+    incremental = True
+    takes_soft = False
+    lag_ok = False    # two rows of one sentence (a live one and a stale one beyond the true count) would write the same slot
+
+    def __init__(self, lm, z, prompts, max_new, page=32):
+        if max_new < 1:
+            raise ValueError('max_new must be at least 1')
+        self.lm, self.V = lm, lm.V
+        dh = lm.d // lm.heads
+        if dh not in (32, 64, 128, 256):
+            raise ValueError('a 4-bit cache needs a head size of 32, 64, 128 or 256, the model has %d' % dh)
+        self.z, toks, lens = _prompt_inputs(lm, z, prompts, 1, max_new - 1)
+        W = lm.prepared()
+        dev, d = lm.device, lm.d
+        B = len(lens)
+        self.R, self.page = B, page
+        self.max_len = max(lens) + max_new - 1
+        i32 = dict(dtype=torch.int32, device=dev)
+        act = dict(dtype=torch.bfloat16 if lm.dtype == 'bf16' else torch.float32, device=dev)
+        f32 = dict(dtype=torch.float32, device=dev)
+        held = [n - 1 for n in lens]                                   # tokens in the cache before the first step
+        need = [-(-(n + max_new) // page) for n in held]
+        self.base = torch.tensor(held, **i32)
+        self.table = torch.empty((B, max(need)), **i32)
+        total = sum(held)
+        cu, used = torch.empty(B + 1, **i32), torch.empty(1, **i32)
+        slots, pos, seq = (torch.empty(total, **i32) for _ in range(3))
+        K.page_plan(self.base, torch.full((B,), max_new, **i32), torch.arange(sum(need), **i32), page, self.table, cu, slots, pos, seq, used)
+        self.caches = [K.Cache4(sum(need), page, lm.heads, dh, dev) for _ in W['layers']]
+        if total > 0:
+            last = torch.tensor(lens).cumsum(0) - 1
+            keep = torch.ones(toks.numel(), dtype=torch.bool)
+            keep[last] = False
+            _run_packed(lm, self.z, toks[keep.to(dev)].contiguous(), pos, seq, cu, total,
+                        lambda li, k, v: K.cache4_write(self.caches[li], k, v, slots, total))
+        self.x, self.h, self.a = torch.empty((B, d), **f32), torch.empty((B, d), **act), torch.empty((B, d), **act)
+        self.ff, self.qkv = torch.empty((B, lm.d_ff), **act), torch.empty((B, 3 * d), **act)
+        self.logits = torch.empty((B, (lm.V + 7) // 8 * 8), **act)
+        work = K.attn_cache4_work(B, lm.heads, lm.heads, dh, self.max_len, dev)
+        layers = [dict(ln_self_g=L['ln1'][0], ln_self_b=L['ln1'][1], wqkv=L['wqkv'], bqkv=L['bqkv'], wo=L['wo'], bo=L['bo'],
+                       ln_ff_g=L['ln2'][0], ln_ff_b=L['ln2'][1], w1=L['w1'], b1=L['b1'], w2=L['w2'], b2=L['b2']) for L in W['layers']]
+        step = K.StepPlan(d=d, heads=lm.heads, d_ff=lm.d_ff, V=self.V, bf16=lm.dtype == 'bf16', n_pos=W['pe'].shape[0], slab_rows=B, S=0, anc_ld=0,
+                          emb=W['emb'], pe=W['pe'], scale=float(torch.tensor(math.sqrt(d), dtype=torch.float32)), z=self.z, mask=None, ln=W['ln'],
+                          wout=W['wout'], bout=W['bout'], x=self.x, h=self.h, q=None, a=self.a, ff=self.ff, logits=self.logits, layers=layers)
+        self.plan = K.PagedPlan(step, self.caches, self.table, self.base, B, self.qkv, work, self.max_len)
+
+    def reorder(self, row_parent, n_rows, identity):
+        pass  # a row finds its pages through its sentence; nothing moves
+
+    def step(self, rows, n, t):
+        """Logits of the next token of rows 0..n-1 (``rows.sent``, ``rows.tok``), each at position base + t of its sentence."""
+        self.plan.run(rows, n, t)
         return self.logits
