@@ -2,9 +2,8 @@
 //
 // A launch is split over groups of adjacent sequences (blockIdx.x) and, within a group, over its tokens (blockIdx.y).  Every
 // workgroup first adds up the tokens and pages of ALL sequences in front of its group: at most a few thousand lengths out of
-// the L2, cheaper than a second launch that would wait for a scan (a launch costs about 2 us, the sum under 1 us at 1000
-// sequences and about 4 us at 8192).  Then it scans its own group in LDS and writes table rows and token entries, consecutive
-// lanes writing consecutive words.
+// the L2, cheaper than a second launch that would wait for a scan.  Then it scans its own group in LDS and writes table rows
+// and token entries; a lane takes four adjacent tokens, one search and three 16-byte stores.
 #include "tst_common.h"
 
 namespace {
@@ -16,83 +15,123 @@ struct PlanArgs {
     int32_t *table, *cu, *slots, *pos, *seq, *used;
     int64_t B, n_pages, N, width;
     int page_shift, group;
+    int aligned_in, aligned_out;    // lens and room / slots, pos and seq start at 16-byte boundaries
 };
 
-__device__ __forceinline__ int64_t tokens_of(const PlanArgs& a, int64_t b) { return max(a.lens[b], 0); }
-__device__ __forceinline__ int64_t need_of(const PlanArgs& a, int64_t b, int64_t tokens) {
-    const int64_t room = a.room != nullptr ? max(a.room[b], 0) : 0;
-    const int64_t need = (tokens + room + (1 << a.page_shift) - 1) >> a.page_shift;
+__device__ __forceinline__ int64_t need_of(const PlanArgs& a, int len, int room) {
+    const int64_t need = ((int64_t)max(len, 0) + max(room, 0) + (1 << a.page_shift) - 1) >> a.page_shift;
     return need < a.width ? need : a.width;
 }
 __device__ __forceinline__ int32_t clip31(int64_t v) { return v > 0x7fffffff ? 0x7fffffff : (int32_t)v; }
 
 __global__ __launch_bounds__(256) void page_plan_kernel(PlanArgs a) {
     __shared__ int64_t part[2][4];
-    __shared__ int64_t tok0[MAX_GROUP + 1], page0[MAX_GROUP + 1];
+    __shared__ int tok0[MAX_GROUP + 1], page0[MAX_GROUP + 1];      // within the group; entries behind its last sequence hold the totals
     const int t = threadIdx.x, lane = t & 63;
     const int64_t b0 = (int64_t)blockIdx.x * a.group;
     const int nb = (int)min((int64_t)a.group, a.B - b0);
     int64_t st = 0, sp = 0;
-    for (int64_t b = t; b < b0; b += 256) {
-        const int64_t n = tokens_of(a, b);
-        st += n;
-        sp += need_of(a, b, n);
+    int64_t b = 0;
+    if (a.aligned_in) {
+        const int64_t quads = b0 >> 2;
+#pragma unroll 4
+        for (int64_t i = t; i < quads; i += 256) {
+            const int4 n = reinterpret_cast<const int4*>(a.lens)[i];
+            const int4 m = a.room != nullptr ? reinterpret_cast<const int4*>(a.room)[i] : make_int4(0, 0, 0, 0);
+            st += (int64_t)max(n.x, 0) + max(n.y, 0) + max(n.z, 0) + max(n.w, 0);
+            sp += need_of(a, n.x, m.x) + need_of(a, n.y, m.y) + need_of(a, n.z, m.z) + need_of(a, n.w, m.w);
+        }
+        b = quads << 2;
+    }
+    for (b += t; b < b0; b += 256) {
+        const int n = a.lens[b];
+        st += max(n, 0);
+        sp += need_of(a, n, a.room != nullptr ? a.room[b] : 0);
     }
     for (int off = 32; off > 0; off >>= 1) {
         st += __shfl_xor(st, off, 64);
         sp += __shfl_xor(sp, off, 64);
     }
     if (lane == 0) { part[0][t >> 6] = st; part[1][t >> 6] = sp; }
-    __syncthreads();
     if (t < 64) {   // scan of the group: one sequence per lane
         int64_t n = 0, p = 0;
         if (lane < nb) {
-            n = tokens_of(a, b0 + lane);
-            p = need_of(a, b0 + lane, n);
+            const int len = a.lens[b0 + lane];
+            n = max(len, 0);
+            p = need_of(a, len, a.room != nullptr ? a.room[b0 + lane] : 0);
         }
         int64_t in = n, ip = p;
         for (int off = 1; off < 64; off <<= 1) {
             const int64_t un = __shfl_up(in, off, 64), up = __shfl_up(ip, off, 64);
             if (lane >= off) { in += un; ip += up; }
         }
-        const int64_t bt = part[0][0] + part[0][1] + part[0][2] + part[0][3], bp = part[1][0] + part[1][1] + part[1][2] + part[1][3];
-        tok0[lane] = bt + in - n;
-        page0[lane] = bp + ip - p;
-        if (lane == 63) { tok0[64] = bt + in; page0[64] = bp + ip; }
+        tok0[lane] = clip31(in - n);
+        page0[lane] = clip31(ip - p);
+        if (lane == 63) { tok0[64] = clip31(in); page0[64] = clip31(ip); }
     }
     __syncthreads();
-    // entries of tok0 / page0 behind the group's last sequence hold the group's totals
-    const int64_t t_end = tok0[MAX_GROUP], p_end = page0[MAX_GROUP];
+    const int64_t t_base = part[0][0] + part[0][1] + part[0][2] + part[0][3], p_base = part[1][0] + part[1][1] + part[1][2] + part[1][3];
     if (blockIdx.y == 0) {
-        if (t < nb) a.cu[b0 + t] = clip31(tok0[t]);
+        if (t < nb) a.cu[b0 + t] = clip31(t_base + tok0[t]);
         if (t == 0 && b0 + nb == a.B) {
-            a.cu[a.B] = clip31(t_end);
-            a.used[0] = clip31(p_end);
+            a.cu[a.B] = clip31(t_base + tok0[MAX_GROUP]);
+            a.used[0] = clip31(p_base + page0[MAX_GROUP]);
         }
     }
     // table rows of the group, entry by entry
     const int64_t cells = (int64_t)nb * a.width;
     for (int64_t i = (int64_t)blockIdx.y * 256 + t; i < cells; i += (int64_t)gridDim.y * 256) {
-        const int s = (int)(i / a.width);
-        const int64_t j = i - (int64_t)s * a.width, at = page0[s] + j;
-        a.table[(b0 + s) * a.width + j] = (at < page0[s + 1] && at < a.n_pages) ? a.pages[at] : -1;
+        const int s = cells <= 0x7fffffff ? (int)((uint32_t)i / (uint32_t)a.width) : (int)(i / a.width);
+        const int64_t j = i - (int64_t)s * a.width, at = p_base + page0[s] + j;
+        a.table[(b0 + s) * a.width + j] = (page0[s] + j < page0[s + 1] && at < a.n_pages) ? a.pages[at] : -1;
     }
-    // tokens of the group
-    const int page = 1 << a.page_shift;
-    const int64_t lo = tok0[0], hi = min(t_end, a.N);
-    for (int64_t i = lo + (int64_t)blockIdx.y * 256 + t; i < hi; i += (int64_t)gridDim.y * 256) {
+    // tokens of the group: lane quads of adjacent tokens, at multiples of four of the packed index
+    const int mask = (1 << a.page_shift) - 1;
+    const int64_t lo = t_base, hi = min(t_base + tok0[MAX_GROUP], a.N);
+    for (int64_t q = (lo >> 2) + (int64_t)blockIdx.y * 256 + t; 4 * q < hi; q += (int64_t)gridDim.y * 256) {
+        const int64_t i0 = max(4 * q, lo);
+        const int r0 = (int)(i0 - lo);
         int s = 0;
-        for (int step = MAX_GROUP / 2; step > 0; step >>= 1)   // the last sequence that starts at or before i and holds it
-            if (s + step < nb && tok0[s + step] <= i) s += step;
-        const int64_t p = i - tok0[s], at = page0[s] + (p >> a.page_shift);
-        int32_t slot = -1;
-        if (at < page0[s + 1] && at < a.n_pages) {
-            const int32_t pg = a.pages[at];
-            if (pg >= 0) slot = clip31(((int64_t)pg << a.page_shift) + (p & (page - 1)));
+        for (int step = MAX_GROUP / 2; step > 0; step >>= 1)   // the last sequence that starts at or before the token: it holds it
+            if (s + step < nb && tok0[s + step] <= r0) s += step;
+        int start = tok0[s], end = tok0[s + 1], pg0 = page0[s], pg1 = page0[s + 1], have = -1, pg = -1;
+        int v_slot[4], v_pos[4], v_seq[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t i = 4 * q + e;
+            v_slot[e] = -1; v_pos[e] = 0; v_seq[e] = 0;
+            if (i < lo || i >= hi) continue;
+            const int r = (int)(i - lo);
+            while (r >= end) {                                 // empty sequences are skipped
+                ++s;
+                start = end; end = tok0[s + 1];
+                pg0 = page0[s]; pg1 = page0[s + 1];
+                have = -1;
+            }
+            const int p = r - start, j = p >> a.page_shift;
+            if (j != have) {
+                const int64_t at = p_base + pg0 + j;
+                pg = (pg0 + j < pg1 && at < a.n_pages) ? a.pages[at] : -1;
+                have = j;
+            }
+            v_slot[e] = pg >= 0 ? clip31(((int64_t)pg << a.page_shift) + (p & mask)) : -1;
+            v_pos[e] = p;
+            v_seq[e] = (int)b0 + s;
         }
-        a.slots[i] = slot;
-        a.pos[i] = (int32_t)p;
-        a.seq[i] = (int32_t)(b0 + s);
+        if (a.aligned_out && 4 * q >= lo && 4 * q + 4 <= hi) {
+            reinterpret_cast<int4*>(a.slots)[q] = make_int4(v_slot[0], v_slot[1], v_slot[2], v_slot[3]);
+            reinterpret_cast<int4*>(a.pos)[q] = make_int4(v_pos[0], v_pos[1], v_pos[2], v_pos[3]);
+            reinterpret_cast<int4*>(a.seq)[q] = make_int4(v_seq[0], v_seq[1], v_seq[2], v_seq[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t i = 4 * q + e;
+                if (i < lo || i >= hi) continue;
+                a.slots[i] = v_slot[e];
+                a.pos[i] = v_pos[e];
+                a.seq[i] = v_seq[e];
+            }
+        }
     }
 }
 
@@ -138,11 +177,12 @@ extern "C" int tst_page_plan(const int32_t* lens, const int32_t* room, int64_t B
                 TST_ERR_ARG, "tst_page_plan: null pointer");
     // groups: small enough to spread the writes over the chip, large enough that the sums in front of the groups stay cheap
     int64_t group = 1;
-    while (group < MAX_GROUP && group * 1024 < B) group *= 2;
+    while (group < MAX_GROUP && group * 512 < B) group *= 2;
     const int64_t groups = B > 0 ? (B + group - 1) / group : 1;
-    int64_t slices = (N + B * width + groups * 2048 - 1) / (groups * 2048);   // about 8 entries per thread
+    int64_t slices = (N + B * width + groups * 4096 - 1) / (groups * 4096);   // about four quads of tokens per thread
     slices = slices < 1 ? 1 : (slices > 1024 ? 1024 : slices);
-    PlanArgs a{lens, room, pages, table, cu, slots, pos, seq, used, B, n_pages, N, width, shift, (int)group};
+    const PlanArgs a{lens, room, pages, table, cu, slots, pos, seq, used, B, n_pages, N, width, shift, (int)group,
+                     tst_aligned16(lens) && tst_aligned16(room), tst_aligned16(slots) && tst_aligned16(pos) && tst_aligned16(seq)};
     page_plan_kernel<<<dim3((unsigned)groups, (unsigned)slices), 256, 0, (hipStream_t)stream>>>(a);
     return tst_after_launch("tst_page_plan");
 }

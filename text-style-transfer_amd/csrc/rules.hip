@@ -3,6 +3,7 @@
 
 namespace {
 
+constexpr int CHUNK_L = 8192, NT_L = 512;   // columns and threads of a workgroup where there are many rows
 constexpr uint32_t SEEN = 0x80000000u;   // counter bit: the token is in the prompt
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -11,19 +12,23 @@ __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const __bf16* p) { return (float)*p; }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(__bf16* p, float v) { *p = (__bf16)v; }
-__device__ __forceinline__ void load16(const float* p, float (&x)[4]) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-}
-__device__ __forceinline__ void load16(const __bf16* p, float (&x)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        x[2 * e] = __uint_as_float(u[e] << 16);
-        x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
+// 16 bytes of logits
+template <typename T>
+struct Piece {
+    uint4 u;
+    __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void values(float (&x)[4]) const {
+        x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y); x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
     }
-}
+    __device__ __forceinline__ void values(float (&x)[8]) const {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[2 * e] = __uint_as_float(w[e] << 16);
+            x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        }
+    }
+};
 __device__ __forceinline__ void store16(float* p, const float (&x)[4]) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
 __device__ __forceinline__ void store16(__bf16* p, const float (&x)[8]) {
     bf16x8 v;
@@ -42,8 +47,8 @@ __device__ __forceinline__ void store16(__bf16* p, const float (&x)[8]) {
 // Chunks begin where the row's addresses are 16-byte aligned, whatever the row's own alignment (`shift` columns before it); a row is only
 // handled element by element where logits and out are aligned differently.  In place (`out` is `logits`), pieces that no rule changes
 // are neither read nor written.
-template <typename T, int CHUNK>
-__global__ __launch_bounds__(256) void adjust_logits_kernel(const T* logits, int64_t ld, int V, tst_logit_rules a, T* out, int64_t ldo) {
+template <typename T, int CHUNK, int NT>
+__global__ __launch_bounds__(NT) void adjust_logits_kernel(const T* logits, int64_t ld, int V, tst_logit_rules a, T* out, int64_t ldo) {
     __shared__ __attribute__((aligned(16))) uint32_t count[CHUNK];
     __shared__ uint16_t list[CHUNK];
     __shared__ int listed;
@@ -68,8 +73,37 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const T* logits, int
         if (a.hist != nullptr) n_hist = a.hist_len != nullptr ? min(a.hist_len[r], (int)a.n_hist) : (int)a.n_hist;
     }
     const bool penal = p_hi > p_lo || n_hist > 0;
+    const int64_t br = a.bias == nullptr ? -1 : (a.bias_row != nullptr ? a.bias_row[r] : 0);
+    const int64_t mr = a.mask == nullptr ? -1 : (a.mask_row != nullptr ? a.mask_row[r] : 0);
+    const float* bias = br >= 0 && br < a.n_bias ? a.bias + br * a.ld_bias : nullptr;
+    const uint32_t* mask = mr >= 0 && mr < a.n_masks ? a.mask + mr * a.ld_mask : nullptr;
+    const int words = (V + 31) >> 5;
+    // the chunk's logits and mask bits are requested before the tokens are counted, unless most of them will not be needed
+    constexpr int PER = CHUNK / E / NT;
+    const bool ahead = out != logits || bias != nullptr;
+    Piece<T> x[PER];
+    uint64_t bits[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int c0 = v0 + (t + NT * j) * E;
+        const bool whole = vec && c0 >= 0 && c0 + E <= V;
+        if (whole && ahead) x[j].load(row_in + c0);
+        bits[j] = ~0ull;
+        if (whole && mask != nullptr) {
+            const int w = c0 >> 5;
+            bits[j] = mask[w];
+            if ((c0 & 31) + E > 32 && w + 1 < words) bits[j] |= (uint64_t)mask[w + 1] << 32;
+        }
+    }
     if (penal) {
-        for (int i = t; i < CHUNK / 4; i += 256) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
+        const int32_t* hist = a.hist + r * a.ld_hist;
+        int vp[4], vh[4];                                            // the first tokens, requested as early
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            vp[u] = p_lo + t + NT * u < p_hi ? a.prompt[p_lo + t + NT * u] : -1;
+            vh[u] = t + NT * u < n_hist ? hist[t + NT * u] : -1;
+        }
+        for (int i = t; i < CHUNK / 4; i += NT) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
         if (t == 0) listed = 0;
         __syncthreads();
         const int lo = max(v0, 0), n = min(v0 + CHUNK, V) - lo;
@@ -78,23 +112,24 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const T* logits, int
             const uint32_t old = prompt ? atomicOr(&count[v - v0], SEEN) : atomicAdd(&count[v - v0], 1u);
             if (old == 0u) list[atomicAdd(&listed, 1)] = (uint16_t)(v - v0);
         };
-        for (int64_t at = (int64_t)p_lo + t; at < p_hi; at += 1024) {
-            int v[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = at + 256 * u < p_hi ? a.prompt[at + 256 * u] : -1;
+        for (int u = 0; u < 4; ++u) note(vp[u], true);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) note(v[u], true);
+        for (int u = 0; u < 4; ++u) note(vh[u], false);
+        for (int64_t at = (int64_t)p_lo + t + 4 * NT; at < p_hi; at += 4 * NT) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) vp[u] = at + NT * u < p_hi ? a.prompt[at + NT * u] : -1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) note(vp[u], true);
         }
-        const int32_t* hist = a.hist + r * a.ld_hist;
-        for (int64_t at = t; at < n_hist; at += 1024) {
-            int v[4];
+        for (int64_t at = t + 4 * NT; at < n_hist; at += 4 * NT) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = at + 256 * u < n_hist ? hist[at + 256 * u] : -1;
+            for (int u = 0; u < 4; ++u) vh[u] = at + NT * u < n_hist ? hist[at + NT * u] : -1;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) note(v[u], false);
+            for (int u = 0; u < 4; ++u) note(vh[u], false);
         }
         __syncthreads();
-        for (int i = t; i < listed; i += 256) {
+        for (int i = t; i < listed; i += NT) {
             const int at = list[i];
             const uint32_t c = count[at];
             float y = load1(row_in + v0 + at);
@@ -104,13 +139,9 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const T* logits, int
         }
         __syncthreads();
     }
-    const int64_t br = a.bias == nullptr ? -1 : (a.bias_row != nullptr ? a.bias_row[r] : 0);
-    const int64_t mr = a.mask == nullptr ? -1 : (a.mask_row != nullptr ? a.mask_row[r] : 0);
-    const float* bias = br >= 0 && br < a.n_bias ? a.bias + br * a.ld_bias : nullptr;
-    const uint32_t* mask = mr >= 0 && mr < a.n_masks ? a.mask + mr * a.ld_mask : nullptr;
-    const int words = (V + 31) >> 5;
-    for (int i = t; i < CHUNK / E; i += 256) {
-        const int c0 = v0 + i * E;                                   // columns c0 .. c0 + E - 1
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = t + NT * j, c0 = v0 + i * E;                  // columns c0 .. c0 + E - 1
         if (c0 >= V) break;
         if (vec && c0 >= 0 && c0 + E <= V) {
             uint32_t n[E], any = 0u;
@@ -122,32 +153,29 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const T* logits, int
                     any |= u.x | u.y | u.z | u.w;
                 }
             }
-            uint32_t allow = (1u << E) - 1u;
-            if (mask != nullptr) {
-                const int w = c0 >> 5;
-                uint64_t bits = mask[w];
-                if ((c0 & 31) + E > 32 && w + 1 < words) bits |= (uint64_t)mask[w + 1] << 32;
-                allow &= (uint32_t)(bits >> (c0 & 31));
+            const uint32_t allow = (uint32_t)(bits[j] >> (c0 & 31)) & ((1u << E) - 1u);
+            if (!ahead) {
+                if (any == 0u && allow == (1u << E) - 1u) continue;
+                x[j].load(row_in + c0);
             }
-            if (out == logits && any == 0u && bias == nullptr && allow == (1u << E) - 1u) continue;
-            float x[E];
-            load16(row_in + c0, x);
+            float y[E];
+            x[j].values(y);
             if (any != 0u) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = n[e] != 0u ? __uint_as_float(~n[e]) : x[e];
+                for (int e = 0; e < E; ++e) y[e] = n[e] != 0u ? __uint_as_float(~n[e]) : y[e];
             }
             if (bias != nullptr) {
 #pragma unroll
                 for (int e = 0; e < E; e += 4) {
                     const float4_any b = *reinterpret_cast<const float4_any*>(bias + c0 + e);
-                    x[e] += b[0]; x[e + 1] += b[1]; x[e + 2] += b[2]; x[e + 3] += b[3];
+                    y[e] += b[0]; y[e + 1] += b[1]; y[e + 2] += b[2]; y[e + 3] += b[3];
                 }
             }
             if (allow != (1u << E) - 1u) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = ((allow >> e) & 1u) != 0u ? x[e] : -INFINITY;
+                for (int e = 0; e < E; ++e) y[e] = ((allow >> e) & 1u) != 0u ? y[e] : -INFINITY;
             }
-            store16(row_out + c0, x);
+            store16(row_out + c0, y);
         } else {
             for (int e = 0; e < E; ++e) {
                 const int v = c0 + e;
@@ -191,8 +219,8 @@ int adjust_logits(const T* logits, int64_t ld, int64_t R, int64_t V, const tst_l
     if (R == 0 || V == 0) return TST_OK;
     TST_REQUIRE(R <= 0x7fffffff / 4, TST_ERR_UNSUPPORTED, "%s: too many rows", who);
     // Long chunks read a row's tokens less often; few rows are cut finer, to have more workgroups than CUs
-    const bool fine = R * ((V + 4095) / 4096) < 512;
-    const int64_t chunk = fine ? 1024 : 4096;
+    const bool fine = R * ((V + CHUNK_L - 1) / CHUNK_L) < 512;
+    const int64_t chunk = fine ? 2048 : CHUNK_L;
     const unsigned chunks = (unsigned)((V + 16 + chunk - 1) / chunk);       // a row may begin up to 7 columns into its first chunk
     for (int64_t r0 = 0; r0 < R; r0 += 65535) {   // grid.y holds at most 65535 rows
         const int64_t n = R - r0 < 65535 ? R - r0 : 65535;
@@ -210,8 +238,8 @@ int adjust_logits(const T* logits, int64_t ld, int64_t R, int64_t V, const tst_l
             }
         }
         const dim3 grid(chunks, (unsigned)n);
-        if (fine) adjust_logits_kernel<T, 1024><<<grid, 256, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
-        else adjust_logits_kernel<T, 4096><<<grid, 256, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
+        if (fine) adjust_logits_kernel<T, 2048, 256><<<grid, 256, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
+        else adjust_logits_kernel<T, CHUNK_L, NT_L><<<grid, NT_L, 0, (hipStream_t)stream>>>(logits + r0 * ld, ld, (int)V, b, out + r0 * ldo, ldo);
         const int rc = tst_after_launch(who);
         if (rc != TST_OK) return rc;
     }
