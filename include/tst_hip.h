@@ -587,7 +587,8 @@ int tst_page_step(const int32_t* base, const int32_t* sent, int64_t t, const int
  * do), out [N][ldo >= heads * dh], which must not overlap them.  Rows outside every sequence are left as they were.  What a row does
  * not attend to never reaches it, NaN and infinities there included.
  * Replaces the self-attention of a model run on whole prefixes (/root/reference/src/inference.py:132).
- * heads % kv_heads == 0; dh <= 256, a multiple of 8 (bf16) or 4 (fp32); leading dimensions likewise, 16-byte aligned pointers.
+ * heads % kv_heads == 0; dh <= 256, a multiple of 8 (bf16) or 4 (fp32); leading dimensions likewise (ldk, ldv <= 2^22), 16-byte
+ * aligned pointers; a finite scale.
  * Scores, softmax and sums are fp32; the bf16 form rounds the weights to bf16 for the product with v, and the result once. */
 int tst_attn_prompt_f32(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv, const int32_t* cu,
                         int64_t B, float* out, int64_t ldo, int64_t N, int64_t heads, int64_t kv_heads, int64_t dh, float scale,
@@ -617,7 +618,8 @@ int tst_cache4_write_f32(const tst_cache4* c, const float* k, int64_t ldk, const
                          int64_t n, void* stream);
 int tst_cache4_write_bf16(const tst_cache4* c, const void* k, int64_t ldk, const void* v, int64_t ldv, const int32_t* slots,
                           int64_t n, void* stream);
-/* Reads rows back as the values the codes stand for (exact in bf16 too, but for E + 2 > 127); a slot outside the cache gives zeros. */
+/* Reads rows back as the values the codes stand for, exact in fp32 and in bf16 (what passes the largest value of the type, codes from 4 on
+ * at E = 126, reads back as infinity); a slot outside the cache gives zeros. */
 int tst_cache4_read_f32(const tst_cache4* c, const int32_t* slots, float* k, int64_t ldk, float* v, int64_t ldv, int64_t n,
                         void* stream);
 int tst_cache4_read_bf16(const tst_cache4* c, const int32_t* slots, void* k, int64_t ldk, void* v, int64_t ldv, int64_t n,

@@ -176,6 +176,24 @@ def test_prompt_large_scores_and_scale(K, dtype):
     check_prompt(q, k, v, cu, out, 2, 1, 64, dtype, scale=3.0)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('size', [1.0, 2.0 ** 100])
+@pytest.mark.parametrize('growth', [0.25, 1.0, 6.0, -1.0])
+@pytest.mark.parametrize('dh', [64, 128, 256])
+def test_prompt_scores_that_outgrow_the_first_tiles(K, dh, growth, size, dtype):
+    """Scores that rise or fall along the keys by up to thousands of powers of two, on values small and near the top of the range."""
+    heads, L = 2, 330
+    g = gen(dh)
+    q, k, v = (torch.randn((L, heads * dh), generator=g, device='cuda') for _ in range(3))
+    for h in range(heads):
+        q[:, h * dh] = 1.0
+        k[:, h * dh] = torch.arange(L, device='cuda') * growth
+    q, k, v = q.to(dtype), k.to(dtype), (v * size).to(dtype)
+    out = torch.empty_like(q)
+    K.attn_prompt(q, k, v, i32([0, L]), out, heads, scale=1.0)
+    check_prompt(q, k, v, [0, L], out, heads, heads, dh, dtype, scale=1.0)
+
+
 def test_prompt_offsets_beyond_32_bits(K):
     buf = torch.empty((33000, 1 << 16), device='cuda', dtype=torch.bfloat16)     # 4.3 GB, 2.16e9 elements
     cu = [32770, 33000]

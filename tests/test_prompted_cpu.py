@@ -33,7 +33,8 @@ def test_attn_prompt_refusals(name, unit):
                       (1, 120, 'hold the heads'), (1, 129, 'hold the heads'), (3, 56, 'hold the heads'), (5, 66, 'hold the heads'), (9, 120, 'hold the heads'),
                       (11, 3, 'hold the heads'), (12, 0, 'multiple of kv_heads'), (11, 0, 'multiple of kv_heads'), (13, unit - 1, 'head size'),
                       (13, 0, 'head size'), (13, 264, 'head size'), (10, -1, 'negative'), (7, -1, 'negative'), (10, 1 << 31, 'exceeds'), (0, 24, '16-byte'),
-                      (8, 20, '16-byte')]:
+                      (8, 20, '16-byte'), (3, (1 << 22) + 64, 'exceeds 2.22'), (5, (1 << 22) + 64, 'exceeds 2.22'), (14, float('nan'), 'not finite'),
+                      (14, float('inf'), 'not finite')]:
         refused(why, name, *(ok[:i] + [v] + ok[i + 1:]))
     refused('multiple of kv_heads', name, *(ok[:11] + [3, 2] + ok[13:]))
     refused('too many', name, *(ok[:1] + [4096 * 8] + ok[2:3] + [4096 * 8] + ok[4:5] + [4096 * 8] + ok[6:9] + [4096 * 8, 1 << 30, 4096, 4096, 8, 0.1, None]))
@@ -56,7 +57,7 @@ def test_cache_refusals(ty):
     for i, v, why in [(0, None, 'null pointer'), (2, None, 'null pointer'), (6, None, 'null pointer'), (8, None, 'null pointer'), (1, 250, 'hold heads'),
                       (9, 128, 'hold heads'), (11, 3, 'multiple of kv_heads'), (11, 0, 'multiple of kv_heads'), (10, -1, 'negative'), (7, -1, 'negative'),
                       (3, -1, 'negative'), (4, -1, 'negative'), (10, 1 << 31, 'exceeds'), (7, 1 << 31, 'exceeds'), (0, 8, '16-byte'), (13, 8, '16-byte'),
-                      (7, 100000, 'are needed')]:
+                      (7, 100000, 'are needed'), (12, float('nan'), 'not finite'), (12, float('-inf'), 'not finite')]:
         refused(why, 'tst_attn_cache4_' + ty, cache(), *(att[:i] + [v] + att[i + 1:]))
 
 

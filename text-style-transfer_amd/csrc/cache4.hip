@@ -706,6 +706,7 @@ int attn_cache4(const tst_cache4* c, const T* q, int64_t ldq, const int32_t* tab
     const int64_t need = tst_attn_cache4_work(R, heads, d.kv_heads, d.dh, max_len);
     TST_REQUIRE(need >= 0 && (need == 0 || (work != nullptr && n_work >= need)), TST_ERR_ARG, "%s: work holds %lld floats, %lld are needed", who,
                 (long long)n_work, (long long)need);
+    TST_REQUIRE(scale - scale == 0.0f, TST_ERR_ARG, "%s: scale is not finite", who);
     if (R == 0) return TST_OK;
     TST_REQUIRE(R * heads <= (int64_t)0x7fffffff, TST_ERR_UNSUPPORTED, "%s: rows * heads exceeds 2^31 - 1", who);
     if (d.slots == 0 || width == 0 || n_seq == 0) max_len = 0;     // nothing can be attended to: zeros
