@@ -82,10 +82,13 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(Cache c, const T* __r
                                                            int64_t ldv, const int32_t* __restrict__ slots, int64_t n) {
     __shared__ __attribute__((aligned(16))) unsigned char tile[TILE_ROWS * RowTile<T>::ROW_BYTES];
     constexpr int E = 16 / (int)sizeof(T), CHUNKS = RowTile<T>::CHUNKS;
-    const bool is_v = blockIdx.z != 0;
+    // columns fastest, so that the workgroups at work read or write whole rows together
+    const int width = c.kv_heads * c.dh, cols = (width + TILE_COLS - 1) / TILE_COLS, col = (int)(blockIdx.x % (unsigned)cols);
+    const unsigned rest = blockIdx.x / (unsigned)cols;
+    const bool is_v = (rest & 1u) != 0;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t i0 = (int64_t)blockIdx.x * TILE_ROWS;
-    const int rows = (int)min((int64_t)TILE_ROWS, n - i0), col0 = blockIdx.y * TILE_COLS, width = c.kv_heads * c.dh;
+    const int64_t i0 = (int64_t)(rest >> 1) * TILE_ROWS;
+    const int rows = (int)min((int64_t)TILE_ROWS, n - i0), col0 = col * TILE_COLS;
     const T* src = is_v ? v + i0 * ldv + col0 : k + i0 * ldk + col0;
     const int64_t ld = is_v ? ldv : ldk;
 #pragma unroll
@@ -95,7 +98,7 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(Cache c, const T* __r
             *reinterpret_cast<uint4*>(tile + r * RowTile<T>::ROW_BYTES + e * (int)sizeof(T)) = *reinterpret_cast<const uint4*>(src + r * ld + e);
     }
     __syncthreads();
-    const int groups = c.dh >> 5, hg = blockIdx.y * 4 + w;
+    const int groups = c.dh >> 5, hg = col * 4 + w;
     if (hg >= c.kv_heads * groups) return;
     const int64_t slot = lane < rows ? slots[i0 + lane] : -1;
     const bool ok = slot >= 0 && slot < c.slots;
@@ -159,11 +162,14 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Cache c, const int32_t
                                                           T* __restrict__ v, int64_t ldv, int64_t n) {
     __shared__ __attribute__((aligned(16))) unsigned char tile[TILE_ROWS * RowTile<T>::ROW_BYTES];
     constexpr int E = 16 / (int)sizeof(T), CHUNKS = RowTile<T>::CHUNKS;
-    const bool is_v = blockIdx.z != 0;
+    // columns fastest, so that the workgroups at work read or write whole rows together
+    const int width = c.kv_heads * c.dh, cols = (width + TILE_COLS - 1) / TILE_COLS, col = (int)(blockIdx.x % (unsigned)cols);
+    const unsigned rest = blockIdx.x / (unsigned)cols;
+    const bool is_v = (rest & 1u) != 0;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t i0 = (int64_t)blockIdx.x * TILE_ROWS;
-    const int rows = (int)min((int64_t)TILE_ROWS, n - i0), col0 = blockIdx.y * TILE_COLS, width = c.kv_heads * c.dh;
-    const int groups = c.dh >> 5, hg = blockIdx.y * 4 + w;
+    const int64_t i0 = (int64_t)(rest >> 1) * TILE_ROWS;
+    const int rows = (int)min((int64_t)TILE_ROWS, n - i0), col0 = col * TILE_COLS;
+    const int groups = c.dh >> 5, hg = col * 4 + w;
     if (hg < c.kv_heads * groups) {
         const int64_t slot = lane < rows ? slots[i0 + lane] : -1;
         const bool ok = slot >= 0 && slot < c.slots;
@@ -665,6 +671,12 @@ int check_rows(const Cache& c, const T* k, int64_t ldk, const T* v, int64_t ldv,
     return TST_OK;
 }
 
+int tile_grid(const Cache& c, int64_t n, int64_t* grid, const char* who) {
+    *grid = (n + TILE_ROWS - 1) / TILE_ROWS * 2 * (((int64_t)c.kv_heads * c.dh + TILE_COLS - 1) / TILE_COLS);
+    TST_REQUIRE(*grid <= (int64_t)0x7fffffff, TST_ERR_UNSUPPORTED, "%s: too many rows", who);
+    return TST_OK;
+}
+
 template <typename T>
 int cache4_write(const tst_cache4* c, const T* k, int64_t ldk, const T* v, int64_t ldv, const int32_t* slots, int64_t n, void* stream,
                  const char* who) {
@@ -672,8 +684,9 @@ int cache4_write(const tst_cache4* c, const T* k, int64_t ldk, const T* v, int64
     int rc = check_cache(c, &d, who);
     if (rc == TST_OK) rc = check_rows(d, k, ldk, v, ldv, slots, n, who);
     if (rc != TST_OK || n == 0) return rc;
-    const dim3 grid((unsigned)((n + TILE_ROWS - 1) / TILE_ROWS), (unsigned)((d.kv_heads * d.dh + TILE_COLS - 1) / TILE_COLS), 2);
-    cache4_write_kernel<T><<<grid, 256, 0, (hipStream_t)stream>>>(d, k, ldk, v, ldv, slots, n);
+    int64_t grid;
+    if ((rc = tile_grid(d, n, &grid, who)) != TST_OK) return rc;
+    cache4_write_kernel<T><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(d, k, ldk, v, ldv, slots, n);
     return tst_after_launch(who);
 }
 
@@ -683,8 +696,9 @@ int cache4_read(const tst_cache4* c, const int32_t* slots, T* k, int64_t ldk, T*
     int rc = check_cache(c, &d, who);
     if (rc == TST_OK) rc = check_rows(d, k, ldk, v, ldv, slots, n, who);
     if (rc != TST_OK || n == 0) return rc;
-    const dim3 grid((unsigned)((n + TILE_ROWS - 1) / TILE_ROWS), (unsigned)((d.kv_heads * d.dh + TILE_COLS - 1) / TILE_COLS), 2);
-    cache4_read_kernel<T><<<grid, 256, 0, (hipStream_t)stream>>>(d, slots, k, ldk, v, ldv, n);
+    int64_t grid;
+    if ((rc = tile_grid(d, n, &grid, who)) != TST_OK) return rc;
+    cache4_read_kernel<T><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(d, slots, k, ldk, v, ldv, n);
     return tst_after_launch(who);
 }
 
