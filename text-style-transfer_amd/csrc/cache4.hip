@@ -51,9 +51,10 @@ __device__ __forceinline__ f32x2 cvt4f(uint32_t codes, uint32_t scale_bits) {
 
 // ---- storing and reading back ---------------------------------------------------------------------------------------------------
 //
-// A workgroup takes 64 rows x 128 elements (4 groups).  Memory sees whole rows of the tile, 16 bytes per lane side by side; between
-// that and the codes the tile passes through LDS, from where each lane (= row) of a wave (= group) reads its 32 elements (rows padded
-// by 16 bytes: 16 lanes fall on 16 different 16-byte places).  Key codes leave as 16 bytes per lane.  Value codes lie token by token:
+// A workgroup takes 64 rows x 128 elements (4 groups).  Memory sees whole rows of the tile, 16 bytes per lane side by side.  Writing, the 4
+// or 8 lanes that hold a group find its scale among them, and only the codes pass through LDS, from where each lane (= row) of a wave
+// (= group) takes its 16 bytes; reading, each lane (= row) writes its 32 elements to LDS and rows leave from there (rows padded by 16
+// bytes: 16 lanes fall on 16 different 16-byte places).  Key codes leave as 16 bytes per lane.  Value codes lie token by token:
 // where the four rows of a lane quad have adjacent slots, the quad transposes its bytes and every lane writes words of four tokens
 // (at any byte address), else single bytes.
 
@@ -77,11 +78,22 @@ __device__ __forceinline__ uint32_t quad_transpose(uint32_t x, int q) {
     return __builtin_amdgcn_perm(z, x, (q & 2) != 0 ? 0x03020706u : 0x05040100u);
 }
 
+// largest of the magnitudes' bits over the LANES lanes that hold a group
+template <int LANES>
+__device__ __forceinline__ uint32_t group_max(uint32_t x) {
+    x = max(x, (uint32_t)lane_xor_i<1>((int)x));
+    x = max(x, (uint32_t)lane_xor_i<2>((int)x));
+    if (LANES == 8) x = max(x, (uint32_t)lane_xor_i<4>((int)x));
+    return x;
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void cache4_write_kernel(Cache c, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v,
                                                            int64_t ldv, const int32_t* __restrict__ slots, int64_t n) {
-    __shared__ __attribute__((aligned(16))) unsigned char tile[TILE_ROWS * RowTile<T>::ROW_BYTES];
-    constexpr int E = 16 / (int)sizeof(T), CHUNKS = RowTile<T>::CHUNKS;
+    constexpr int E = 16 / (int)sizeof(T), CHUNKS = RowTile<T>::CHUNKS, PER = TILE_ROWS * CHUNKS / 256;
+    constexpr int CODE_ROW = TILE_COLS / 2 + 16;                           // bytes of codes per row, padded
+    __shared__ __attribute__((aligned(16))) unsigned char code_tile[TILE_ROWS * CODE_ROW];
+    __shared__ uint32_t scale_tile[TILE_ROWS];                             // the four groups' scale bytes
     // columns fastest, so that the workgroups at work read or write whole rows together
     const int width = c.kv_heads * c.dh, cols = (width + TILE_COLS - 1) / TILE_COLS, col = (int)(blockIdx.x % (unsigned)cols);
     const unsigned rest = blockIdx.x / (unsigned)cols;
@@ -91,42 +103,48 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(Cache c, const T* __r
     const int rows = (int)min((int64_t)TILE_ROWS, n - i0), col0 = col * TILE_COLS;
     const T* src = is_v ? v + i0 * ldv + col0 : k + i0 * ldk + col0;
     const int64_t ld = is_v ? ldv : ldk;
+    uint4 in[PER];
 #pragma unroll
-    for (int j = 0; j < TILE_ROWS * CHUNKS / 256; ++j) {
+    for (int j = 0; j < PER; ++j) {
         const int x = threadIdx.x + 256 * j, r = x / CHUNKS, e = (x % CHUNKS) * E;
-        if (r < rows && col0 + e < width)
-            *reinterpret_cast<uint4*>(tile + r * RowTile<T>::ROW_BYTES + e * (int)sizeof(T)) = *reinterpret_cast<const uint4*>(src + r * ld + e);
+        in[j] = *reinterpret_cast<const uint4*>(src + min(r, rows - 1) * ld + (col0 + e < width ? e : 0));    // what is not there goes nowhere
+    }
+    const int64_t slot = lane < rows ? slots[i0 + lane] : -1;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int x = threadIdx.x + 256 * j, r = x / CHUNKS, ch = x % CHUNKS;
+        const uint4 u = in[j];
+        float y[E];
+        if (E == 4) {
+            y[0] = __uint_as_float(u.x); y[1] = __uint_as_float(u.y); y[2] = __uint_as_float(u.z); y[3] = __uint_as_float(u.w);
+        } else {
+            y[0] = low_f(u.x); y[1] = high_f(u.x); y[2] = low_f(u.y); y[3] = high_f(u.y);
+            y[E - 4] = low_f(u.z); y[E - 3] = high_f(u.z); y[E - 2] = low_f(u.w); y[E - 1] = high_f(u.w);
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
+        const int s = scale_byte(group_max<32 / E>(top));
+        const float unit = __uint_as_float(scale_to_bits(s == 255 ? 127 : s));
+        // x * 2^-E, rounded to the nearest code, ties to the even one
+        uint32_t codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], unit, 0);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[2], y[3], unit, 1);
+        if (E == 8) {
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[E - 4], y[E - 3], unit, 2);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[E - 2], y[E - 1], unit, 3);
+            *reinterpret_cast<uint32_t*>(code_tile + r * CODE_ROW + 4 * ch) = codes;
+        } else {
+            *reinterpret_cast<uint16_t*>(code_tile + r * CODE_ROW + 2 * ch) = (uint16_t)codes;
+        }
+        if ((ch & (32 / E - 1)) == 0) reinterpret_cast<uint8_t*>(scale_tile)[4 * r + ch / (32 / E)] = (uint8_t)s;
     }
     __syncthreads();
     const int groups = c.dh >> 5, hg = col * 4 + w;
     if (hg >= c.kv_heads * groups) return;
-    const int64_t slot = lane < rows ? slots[i0 + lane] : -1;
     const bool ok = slot >= 0 && slot < c.slots;
-    const unsigned char* mine = tile + (lane < rows ? lane : 0) * RowTile<T>::ROW_BYTES + w * 32 * (int)sizeof(T);
-    float x[32];
-#pragma unroll
-    for (int e = 0; e < 32; e += E) {
-        const uint4 u = *reinterpret_cast<const uint4*>(mine + e * (int)sizeof(T));
-        if (E == 4) {
-            x[e] = __uint_as_float(u.x); x[e + 1] = __uint_as_float(u.y); x[e + 2] = __uint_as_float(u.z); x[e + 3] = __uint_as_float(u.w);
-        } else {
-            x[e] = low_f(u.x); x[e + 1] = high_f(u.x); x[e + 2] = low_f(u.y); x[e + 3] = high_f(u.y);
-            x[e + E - 4] = low_f(u.z); x[e + E - 3] = high_f(u.z); x[e + E - 2] = low_f(u.w); x[e + E - 1] = high_f(u.w);
-        }
-    }
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 32; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-    const int s = scale_byte(top);
-    const float unit = __uint_as_float(scale_to_bits(s == 255 ? 127 : s));
-    uint32_t codes[4];
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {   // x * 2^-E, rounded to the nearest code, ties to the even one
-        codes[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[8 * d], x[8 * d + 1], unit, 0);
-        codes[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes[d], x[8 * d + 2], x[8 * d + 3], unit, 1);
-        codes[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes[d], x[8 * d + 4], x[8 * d + 5], unit, 2);
-        codes[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes[d], x[8 * d + 6], x[8 * d + 7], unit, 3);
-    }
+    const uint4 mine = *reinterpret_cast<const uint4*>(code_tile + lane * CODE_ROW + 16 * w);
+    const uint32_t codes[4] = {mine.x, mine.y, mine.z, mine.w};
+    const int s = (int)(scale_tile[lane] >> (8 * w) & 255u);
     const int h = hg / groups, g = hg - h * groups;
     const int page = 1 << c.page_shift, tok = (int)slot & (page - 1);
     const int64_t ph = (ok ? slot >> c.page_shift : 0) * c.kv_heads + h;
