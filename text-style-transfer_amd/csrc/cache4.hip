@@ -589,16 +589,33 @@ __global__ __launch_bounds__(512) void attn_cache4_combine_kernel(AttendArgs a) 
     __shared__ float part[8][64 * E + 1];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t r = blockIdx.x / (uint32_t)a.heads, head = blockIdx.x - r * a.heads;
+    const float* ml = a.work + 2 * (r * a.heads + head) * a.splits;
+    const float* op = a.work + 2 * a.R * a.heads * a.splits + (r * a.heads + head) * a.splits * DH;
+    // a block of AHEAD chunks: maxima, sums and outputs, requested before the row's length is known (what lies behind it is not used)
+    constexpr int AHEAD = 8;
+    f32x2 head_ml[AHEAD];
+    float piece[AHEAD][E];
+    const int el = min(lane * E, DH - E);
+    auto request = [&](int i0, int end) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int64_t i = min(i0 + w + 8 * u, end - 1);
+            head_ml[u] = *reinterpret_cast<const f32x2*>(ml + 2 * i);
+#pragma unroll
+            for (int e = 0; e < E; ++e) piece[u][e] = op[i * DH + el + e];
+        }
+    };
+    request(0, a.splits);
+    const f32x2 mine = *reinterpret_cast<const f32x2*>(ml + 2 * min(lane, a.splits - 1));
     const int64_t s = a.seq != nullptr ? a.seq[r] : r;
     int64_t len = s >= 0 && s < a.n_seq ? a.lens[r] : 0;
     len = max(min(min(len, a.max_len), a.width << a.c.page_shift), (int64_t)0);
     if (len <= a.chunk) return;
     const int n = (int)((len + a.chunk - 1) / a.chunk);
-    const float* ml = a.work + 2 * (r * a.heads + head) * a.splits;
-    const float* op = a.work + 2 * a.R * a.heads * a.splits + (r * a.heads + head) * a.splits * DH;
     float m = -INFINITY;
     bool some = false;
-    for (int i = lane; i < n; i += 64)
+    if (lane < n && !(mine[1] < 0.0f)) { m = mine[0]; some = true; }
+    for (int i = lane + 64; i < n; i += 64)
         if (!(ml[2 * i + 1] < 0.0f)) { m = fmaxf(m, ml[2 * i]); some = true; }
     m = wave_max(m);
     some = __ballot(some) != 0ull;
@@ -606,14 +623,18 @@ __global__ __launch_bounds__(512) void attn_cache4_combine_kernel(AttendArgs a) 
     float acc[E], sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-    for (int i = w; i < n; i += 8) {
-        const float si = ml[2 * i + 1];
-        const float f = si < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * i] - base);
-        sum += si < 0.0f ? 0.0f : si * f;
+    for (int i0 = 0;;) {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (lane * E + e < DH) acc[e] += op[(int64_t)i * DH + lane * E + e] * f;    // a chunk without tokens holds zeros
+        for (int u = 0; u < AHEAD; ++u) {
+            const float si = head_ml[u][1];
+            if (i0 + w + 8 * u >= n || si < 0.0f) continue;              // behind the row, or a chunk without tokens
+            const float f = __builtin_amdgcn_exp2f(head_ml[u][0] - base);
+            sum += si * f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += piece[u][e] * f;
+        }
+        if ((i0 += 8 * AHEAD) >= n) break;
+        request(i0, n);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) part[w][lane * E + e] = acc[e];
