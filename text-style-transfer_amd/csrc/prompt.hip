@@ -51,10 +51,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) { return __builtin_b
 __device__ __forceinline__ float low_f(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float high_f(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
-// what a piece that rounds x leaves over; a piece that is infinite or NaN is the whole value
-__device__ __forceinline__ float rest(float x, float piece) { return (__float_as_uint(piece) & 0x7f800000u) == 0x7f800000u ? 0.0f : x - piece; }
-
-// eight elements as NP pieces of eight bf16
+// Eight elements as NP pieces of eight bf16.  What is not finite, or rounds to infinity, leaves a NaN in the second piece, which every product
+// passes on: rows that meet it are computed again, plainly.
 __device__ __forceinline__ void split8(const float (&x)[8], bool negate, Frag (&f)[3]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -62,8 +60,8 @@ __device__ __forceinline__ void split8(const float (&x)[8], bool negate, Frag (&
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
             f[i].u[e] = pack2(a, b);
-            a = rest(a, low_f(f[i].u[e]));
-            b = rest(b, high_f(f[i].u[e]));
+            a = a - low_f(f[i].u[e]);
+            b = b - high_f(f[i].u[e]);
         }
     }
 }
@@ -297,10 +295,10 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
                     for (int e = 0; e < 4; ++e) {
                         f.u[e] = pack2(x8[2 * e], x8[2 * e + 1]);
                         d.u[e] = pack2(y8[2 * e], y8[2 * e + 1]);
-                        x8[2 * e] = rest(x8[2 * e], low_f(f.u[e]));
-                        x8[2 * e + 1] = rest(x8[2 * e + 1], high_f(f.u[e]));
-                        y8[2 * e] = rest(y8[2 * e], low_f(d.u[e]));
-                        y8[2 * e + 1] = rest(y8[2 * e + 1], high_f(d.u[e]));
+                        x8[2 * e] = x8[2 * e] - low_f(f.u[e]);
+                        x8[2 * e + 1] = x8[2 * e + 1] - high_f(f.u[e]);
+                        y8[2 * e] = y8[2 * e] - low_f(d.u[e]);
+                        y8[2 * e + 1] = y8[2 * e + 1] - high_f(d.u[e]);
                     }
                     *reinterpret_cast<uint4*>(dk + i * PLANE) = f.q;
                     *reinterpret_cast<uint4*>(dv + i * PLANE) = d.q;
