@@ -672,3 +672,71 @@ def test_prefill_then_steps(K, dtype):
     for t in range(steps):
         vals = [quantise64(torch.cat([qkv[at[i]:at[i + 1], a:], new[:t + 1, i, a:]])) for i in range(B)]
         check_attend(new[t, :, :a], vals, [n + t + 1 for n in lens], res[t], heads, kv_heads, dh, dtype)
+
+
+# ---- all of them together --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_a_step_of_all_operators_captured_and_replayed(K, dtype):
+    """Plan, prompt attention, cache, one decode step, rules and grammar in one graph on a stream of its own: replays over new inputs, with
+    eager work between them, give the bits of eager calls."""
+    heads, kv_heads, dh, page, V, B, states = 4, 2, 64, 32, 1003, 5, 4
+    wq, wk = heads * dh, kv_heads * dh
+    width, N = 8, 700
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        lens = torch.randint(0, 140, (B,), generator=g)
+        lens[seed % B] = 0
+        d = dict(lens=lens.int(), room=torch.full((B,), 3, dtype=torch.int32), pages=torch.randperm(B * width, generator=g).int(),
+                 qkv=torch.randn((N, wq + 2 * wk), generator=g).to(dtype), step=torch.randn((B, wq + 2 * wk), generator=g).to(dtype),
+                 logits=torch.randn((B, V), generator=g).to(dtype), hist=torch.randint(0, V, (B, 9), generator=g).int(),
+                 params=torch.rand((B, 3), generator=g) + 0.5, bias=torch.randn((1, V), generator=g),
+                 mask=torch.randint(-2 ** 31, 2 ** 31 - 1, (states, (V + 31) // 32), generator=g).int(),
+                 state=torch.randint(0, states, (B,), generator=g).int(), tok=torch.randint(0, V, (B,), generator=g).int(),
+                 next=torch.randint(-1, states, (states, V), generator=g).int())
+        return {k: v.cuda() for k, v in d.items()}
+
+    def buffers():
+        z = lambda *s, t=torch.int32: torch.zeros(s, dtype=t, device='cuda')       # noqa: E731
+        return dict(table=z(B, width), cu=z(B + 1), slots=z(N), pos=z(N), seq=z(N), used=z(1), out=z(N, wq, t=dtype), s_slots=z(B), s_pos=z(B),
+                    s_lens=z(B), att=z(B, wq, t=dtype), y=z(B, V, t=dtype), after=z(B), cache=K.Cache4(B * width, page, kv_heads, dh),
+                    work=K.attn_cache4_work(B, heads, kv_heads, dh, width * page, 'cuda'))
+
+    def run(i, b):
+        K.page_plan(i['lens'], i['room'], i['pages'], page, b['table'], b['cu'], b['slots'], b['pos'], b['seq'], b['used'])
+        q, k, v = i['qkv'][:, :wq], i['qkv'][:, wq:wq + wk], i['qkv'][:, wq + wk:]
+        K.attn_prompt(q, k, v, b['cu'], b['out'], heads, kv_heads)
+        K.cache4_write(b['cache'], k, v, b['slots'], N)
+        K.page_step(i['lens'], None, 0, b['table'], page, b['s_slots'], b['s_pos'], b['s_lens'], B)
+        K.cache4_write(b['cache'], i['step'][:, wq:wq + wk], i['step'][:, wq + wk:], b['s_slots'], B)
+        K.attn_cache4(i['step'][:, :wq], b['cache'], b['table'], b['s_lens'], b['att'], B, heads, width * page, work=b['work'])
+        K.adjust_logits(i['logits'], B, V, b['y'], params=i['params'], hist=i['hist'], bias=i['bias'], mask=i['mask'], mask_row=i['state'])
+        K.grammar_next(i['next'], i['state'], None, i['tok'], b['after'], B)
+
+    fixed, mine = inputs(0), buffers()
+    mine['slots'].fill_(-1)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run(fixed, mine)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        run(fixed, mine)
+    names = ('table', 'cu', 'used', 's_slots', 's_pos', 's_lens', 'att', 'y', 'after')
+    for seed in (3, 1, 2, 3):
+        new, plain = inputs(seed), buffers()
+        plain['slots'].fill_(-1)
+        run(new, plain)
+        mine['slots'].fill_(-1)                          # entries behind the last token stay as they are: no slot
+        for k in fixed:
+            fixed[k].copy_(new[k])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        n = int(plain['cu'][-1])
+        for k in names:
+            assert torch.equal(mine[k], plain[k]), (seed, k)
+        for k in ('slots', 'pos', 'seq', 'out'):
+            assert torch.equal(mine[k][:n], plain[k][:n]), (seed, k)
+        assert n == int(new['lens'].sum()) and not torch.isnan(mine['att'].float()).any()
