@@ -632,13 +632,14 @@ def retire_compact(cur, nxt, sel, lp, n_sent, k, step, T, eos, last_step, top_en
 
 _I32, _U8, _F32, _BF16 = torch.int32, torch.uint8, torch.float32, torch.bfloat16
 _device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)
+_stream_of = _raw_stream if _raw_stream is not None else lambda dev: torch.cuda.current_stream(dev).cuda_stream
 
 
 # The checks below run on every call of kernels that take a few microseconds: each asks a tensor for as little as it can.  All tensors
 # have to live on the current device, on whose current stream the kernels run (``dev``: its number; a CPU tensor answers -1).
 
 def _rows2d(t, dtype, dev, n_rows, n_cols, name):
-    """Leading dimension of a 2-D view whose rows the kernels can read 16 bytes at a time."""
+    """(address, leading dimension) of a 2-D view whose rows the kernels can read 16 bytes at a time."""
     shape, stride = t.shape, t.stride()
     if t.dtype is not dtype or len(shape) != 2 or t.get_device() != dev or (stride[1] != 1 and shape[1] > 1):
         raise ValueError('%s must be a 2-D %s tensor with unit inner stride on the current GPU, got %s %s on %s'
@@ -652,16 +653,17 @@ def _rows2d(t, dtype, dev, n_rows, n_cols, name):
         ld += -ld % unit
     elif ld < n_cols or ld % unit:
         raise ValueError('rows of %s must not overlap and start at multiples of %d elements (16 bytes)' % (name, unit))
-    if t.data_ptr() % 16:
+    at = t.data_ptr()
+    if at & 15:
         raise ValueError('%s must start at a 16-byte boundary' % name)
-    return ld
+    return at, ld
 
 
 def _ints(t, n, dev, name):
     """Address of a 1-D int32 tensor of at least n entries (None: a null pointer)."""
     if t is None:
         return None
-    if t.dtype is not _I32 or t.dim() != 1 or t.numel() < n or t.get_device() != dev or not t.is_contiguous():
+    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
         raise ValueError('%s must be a contiguous int32 tensor [%d] on the current GPU, got %s %s on %s' % (name, n, t.dtype, tuple(t.shape), t.device))
     return t.data_ptr()
 
@@ -696,13 +698,13 @@ def attn_prompt(q, k, v, cu, out, heads, kv_heads=None, scale=None):
     if dh % unit or not 0 < dh <= 256:
         raise ValueError('head size %d is not a multiple of %d up to 256' % (dh, unit))
     wk = kv_heads * dh
-    ldq, ldk = _rows2d(q, dt, dev, N, wq, 'q'), _rows2d(k, dt, dev, N, wk, 'k')
-    ldv, ldo = _rows2d(v, dt, dev, N, wk, 'v'), _rows2d(out, dt, dev, N, wq, 'out')
-    pq, pk, pv, po, pc = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ints(cu, 1, dev, 'cu')
+    (pq, ldq), (pk, ldk) = _rows2d(q, dt, dev, N, wq, 'q'), _rows2d(k, dt, dev, N, wk, 'k')
+    (pv, ldv), (po, ldo) = _rows2d(v, dt, dev, N, wk, 'v'), _rows2d(out, dt, dev, N, wq, 'out')
+    pc = _ints(cu, 1, dev, 'cu')
     for p, ld, w in ((pq, ldq, wq), (pk, ldk, wk), (pv, ldv, wk)):
         _disjoint(po, ldo, p, ld, N, wq, w, size, 'out must not overlap q, k or v')
     call('tst_attn_prompt_bf16' if dt is _BF16 else 'tst_attn_prompt_f32', pq, ldq, pk, ldk, pv, ldv, pc, cu.numel() - 1, po, ldo, N, heads, kv_heads,
-         dh, dh ** -0.5 if scale is None else scale, _stream())
+         dh, dh ** -0.5 if scale is None else scale, _stream_of(dev))
 
 
 def page_plan(lens, room, pages, page, table, cu, slots, pos, seq, used):
@@ -719,7 +721,7 @@ def page_plan(lens, room, pages, page, table, cu, slots, pos, seq, used):
         raise ValueError('pages * page exceeds 2^31 - 1: slots are 32-bit')
     call('tst_page_plan', _ints(lens, B, dev, 'lens'), _ints(room, B, dev, 'room'), B, _ints(pages, 0, dev, 'pages'), n_pages, page, table.data_ptr(),
          width, _ints(cu, B + 1, dev, 'cu'), _ints(slots, N, dev, 'slots'), _ints(pos, N, dev, 'pos'), _ints(seq, N, dev, 'seq'), N,
-         _ints(used, 1, dev, 'used'), _stream())
+         _ints(used, 1, dev, 'used'), _stream_of(dev))
 
 
 def page_step(base, sent, t, table, page, slots, pos, lens, n_rows):
@@ -728,7 +730,7 @@ def page_step(base, sent, t, table, page, slots, pos, lens, n_rows):
     dev = _device()
     n_seq, width = _table(table, dev, 'table')
     call('tst_page_step', _ints(base, n_seq, dev, 'base'), _ints(sent, n_rows, dev, 'sent'), t, table.data_ptr(), width, n_seq, page,
-         _ints(slots, n_rows, dev, 'slots'), _ints(pos, n_rows, dev, 'pos'), _ints(lens, n_rows, dev, 'lens'), n_rows, _stream())
+         _ints(slots, n_rows, dev, 'slots'), _ints(pos, n_rows, dev, 'pos'), _ints(lens, n_rows, dev, 'lens'), n_rows, _stream_of(dev))
 
 
 class Cache4:
@@ -769,8 +771,8 @@ def cache4_write(cache, k, v, slots, n_rows):
     dt, w, dev = k.dtype, cache.kv_heads * cache.dh, _device()
     if dt is not _BF16 and dt is not _F32:
         raise ValueError('rows must be fp32 or bf16')
-    call('tst_cache4_write_bf16' if dt is _BF16 else 'tst_cache4_write_f32', cache._on(dev), k.data_ptr(), _rows2d(k, dt, dev, n_rows, w, 'k'), v.data_ptr(),
-         _rows2d(v, dt, dev, n_rows, w, 'v'), _ints(slots, n_rows, dev, 'slots'), n_rows, _stream())
+    call('tst_cache4_write_bf16' if dt is _BF16 else 'tst_cache4_write_f32', cache._on(dev), *_rows2d(k, dt, dev, n_rows, w, 'k'),
+         *_rows2d(v, dt, dev, n_rows, w, 'v'), _ints(slots, n_rows, dev, 'slots'), n_rows, _stream_of(dev))
 
 
 def cache4_read(cache, slots, k, v, n_rows):
@@ -778,8 +780,8 @@ def cache4_read(cache, slots, k, v, n_rows):
     dt, w, dev = k.dtype, cache.kv_heads * cache.dh, _device()
     if dt is not _BF16 and dt is not _F32:
         raise ValueError('rows must be fp32 or bf16')
-    call('tst_cache4_read_bf16' if dt is _BF16 else 'tst_cache4_read_f32', cache._on(dev), _ints(slots, n_rows, dev, 'slots'), k.data_ptr(),
-         _rows2d(k, dt, dev, n_rows, w, 'k'), v.data_ptr(), _rows2d(v, dt, dev, n_rows, w, 'v'), n_rows, _stream())
+    call('tst_cache4_read_bf16' if dt is _BF16 else 'tst_cache4_read_f32', cache._on(dev), _ints(slots, n_rows, dev, 'slots'),
+         *_rows2d(k, dt, dev, n_rows, w, 'k'), *_rows2d(v, dt, dev, n_rows, w, 'v'), n_rows, _stream_of(dev))
 
 
 def attn_cache4_work(n_rows, heads, kv_heads, head_size, max_len, device='cuda'):
@@ -801,8 +803,7 @@ def attn_cache4(q, cache, table, lens, out, n_rows, heads, max_len, seq=None, sc
     if heads < 1 or heads % cache.kv_heads:
         raise ValueError("heads must be a multiple of the cache's %d" % cache.kv_heads)
     w = heads * dh
-    ldq, ldo = _rows2d(q, dt, dev, n_rows, w, 'q'), _rows2d(out, dt, dev, n_rows, w, 'out')
-    pq, po = q.data_ptr(), out.data_ptr()
+    (pq, ldq), (po, ldo) = _rows2d(q, dt, dev, n_rows, w, 'q'), _rows2d(out, dt, dev, n_rows, w, 'out')
     _disjoint(po, ldo, pq, ldq, n_rows, w, w, 2 if dt is _BF16 else 4, 'out must not overlap q')
     n_seq, width = _table(table, dev, 'table')
     if work is None:
@@ -811,7 +812,7 @@ def attn_cache4(q, cache, table, lens, out, n_rows, heads, max_len, seq=None, sc
         raise ValueError('work must be a contiguous fp32 tensor on the current GPU')
     call('tst_attn_cache4_bf16' if dt is _BF16 else 'tst_attn_cache4_f32', cache._on(dev), pq, ldq, table.data_ptr(), width, n_seq,
          _ints(seq, n_rows, dev, 'seq'), _ints(lens, n_rows, dev, 'lens'), max_len, po, ldo, n_rows, heads, dh ** -0.5 if scale is None else scale,
-         None if work is None else work.data_ptr(), 0 if work is None else work.numel(), _stream())
+         None if work is None else work.data_ptr(), 0 if work is None else work.numel(), _stream_of(dev))
 
 
 def _rule_rows(t, dtype, width, dev, name):
@@ -872,7 +873,7 @@ def adjust_logits(logits, n_rows, n_cols, out, *, params=None, sent=None, hist=N
     if mask is not None:
         rules.mask, rules.ld_mask, rules.n_masks = _rule_rows(mask, _I32, (n_cols + 31) // 32, dev, 'mask')
         rules.mask_row = _ints(mask_row, n_rows, dev, 'mask_row')
-    call('tst_adjust_logits_bf16' if dt is _BF16 else 'tst_adjust_logits_f32', p_in, lds[0], n_rows, n_cols, rules, p_out, lds[1], _stream())
+    call('tst_adjust_logits_bf16' if dt is _BF16 else 'tst_adjust_logits_f32', p_in, lds[0], n_rows, n_cols, rules, p_out, lds[1], _stream_of(dev))
 
 
 def grammar_next(table, state, parent, tok, out, n_rows):
@@ -883,7 +884,7 @@ def grammar_next(table, state, parent, tok, out, n_rows):
     if po == ps:
         raise ValueError('out must not be state')
     call('tst_grammar_next', table.data_ptr(), n_states, V, ps, state.numel(), _ints(parent, n_rows, dev, 'parent'), _ints(tok, n_rows, dev, 'tok'), po, n_rows,
-         _stream())
+         _stream_of(dev))
 
 
 class PagedPlan:
