@@ -99,17 +99,18 @@ __device__ __forceinline__ void dma16(uint32_t lds, const void* base, uint32_t o
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
-// LDS tiles are rows of DH / 8 chunks of 16 bytes.  Chunk c of row r sits at place c ^ swizzle(r), so that the 16 rows that a key fragment
-// reads at one c, and the 8 rows x 4 chunks that a value fragment reads, fall on different banks.
+// LDS tiles are rows of DH / 8 chunks of 16 bytes.  Chunk c of row r sits at place c ^ swizzle(r), so that what an LDS read fetches in one
+// clock falls on different banks, whether that is 128 bytes of 32 banks or 256 of 64: 8 or 16 rows at one chunk for a key fragment, 4
+// rows at 2 or 4 chunks for a value fragment.  (Rows of 256 bytes or more: all rows start at bank 0; of 128: every second; of 64: fourth.)
 template <int DH>
 __device__ __forceinline__ int k_swizzle(int r) {
-    constexpr int CH = DH / 8, RW = CH >= 16 ? 1 : 16 / CH;
-    return (r / RW) & ((CH < 16 ? CH : 16) - 1);
+    constexpr int CH = DH / 8;
+    return CH >= 16 ? r & 15 : (CH == 8 ? (r & 6) | ((r ^ (r >> 3)) & 1) : (((r >> 1) ^ (r >> 3)) & 1) | ((r >> 1) & 2));
 }
 template <int DH>
 __device__ __forceinline__ int v_swizzle(int r) {
     constexpr int CH = DH / 8;
-    return CH >= 16 ? 2 * (r & 7) : (CH == 8 ? 2 * ((r >> 1) & 3) : 0);
+    return CH >= 16 ? 2 * (r & 3) + 8 * (r & 1) : (CH == 8 ? 2 * (r & 3) : r & 2);
 }
 
 // One query row by one wave, plainly, reading nothing that the row does not attend to: for rows whose fast result is NaN, because a
