@@ -57,6 +57,8 @@ __device__ __forceinline__ f32x2 cvt4f(uint32_t codes, uint32_t scale_bits) {
 // bytes: 16 lanes fall on 16 different 16-byte places).  Key codes leave as 16 bytes per lane.  Value codes lie token by token:
 // where the four rows of a lane quad have adjacent slots, the quad transposes its bytes and every lane writes words of four tokens
 // (at any byte address), else single bytes.
+// Bound by memory: 65521 rows of 8 heads of 128 in fp32 are stored in 142 us (608 MB, 4.3 TB/s) and read back in 114 (5.3 TB/s; a copy of 2
+// GB runs at 4.9).  With rows of 512 bytes at a time, column tiles slowest, it was 175 and 135; through LDS in fp32, 168 to store.
 
 constexpr int TILE_ROWS = 64, TILE_COLS = 128;
 
@@ -248,7 +250,8 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Cache c, const int32_t
 // accuracy at three matrix instructions instead of one.  bf16 queries are one piece, and the weights are rounded to bf16 (half a step,
 // 2^-9 of a weight in [2^k, 2^(k+1)), against an output of 8 bits).
 //
-// Long contexts are split over workgroups (rows x key heads x chunks) and, inside one, over its waves (tile by tile in turn); partial
+// Bound by memory: 256 rows of 8 key heads of 128, contexts of up to 8000 tokens (1.09 GB): 219 us, 5.0 TB/s, matrix instructions busy a
+// seventh of the time.  Long contexts are split over workgroups (rows x key heads x chunks) and, inside one, over its waves (tile by tile in turn); partial
 // (maximum, sum, O) are joined in LDS and by combine_kernel, in a fixed order.
 
 union Frag {
@@ -657,7 +660,7 @@ __global__ __launch_bounds__(512) void attn_cache4_combine_kernel(AttendArgs a) 
 
 // How a call is cut: tokens per workgroup (chunk) and how many chunks the longest row may have.  Few (row, key head) units: as many
 // workgroups as run at once, two to a CU, since every chunk costs a prologue and a partial result (3 rows x 4 key heads, 131001
-// tokens: 38.8 us at 512 workgroups, 41.5 at 1024, 46.7 at 1536).  Many: 1024, so that rows of different lengths even out, and whole
+// tokens: 36.8 us at 512 workgroups; before the partial results were requested early 38.8, 41.5 at 1024, 46.7 at 1536).  Many: 1024, so that rows of different lengths even out, and whole
 // rows up to 8192 tokens once there are that many units (256 rows x 8 key heads, up to 8000 tokens: 219 us in one piece, 225 cut at
 // 4096, 231 at 2048).  At least one tile for each of the four waves.
 void cut(int64_t R, int64_t kv_heads, int64_t head_groups, int64_t max_len, int* chunk, int* splits) {

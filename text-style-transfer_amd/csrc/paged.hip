@@ -4,6 +4,8 @@
 // workgroup first adds up the tokens and pages of ALL sequences in front of its group: at most a few thousand lengths out of
 // the L2, cheaper than a second launch that would wait for a scan.  Then it scans its own group in LDS and writes table rows
 // and token entries; a lane takes four adjacent tokens, one search and three 16-byte stores.
+// 8192 sequences, 2.1 M tokens (27 MB): 12.2 us, 18.8 with one token per lane; 48 sequences: 5.2 us, a launch and the chain of loads
+// lengths -> offsets -> pages.
 #include "tst_common.h"
 
 namespace {
