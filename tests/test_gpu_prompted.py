@@ -740,3 +740,81 @@ def test_a_step_of_all_operators_captured_and_replayed(K, dtype):
         for k in ('slots', 'pos', 'seq', 'out'):
             assert torch.equal(mine[k][:n], plain[k][:n]), (seed, k)
         assert n == int(new['lens'].sum()) and not torch.isnan(mine['att'].float()).any()
+
+
+# ---- what the wrappers refuse (nothing is launched) -----------------------------------------------------------------------------------
+def test_wrappers_refuse(K):
+    from tst_amd import TstError
+    z = lambda *s, t=torch.float32: torch.zeros(s, dtype=t, device='cuda')            # noqa: E731
+    iz = lambda *s: z(*s, t=torch.int32)                                               # noqa: E731
+    rows = z(8, 256)
+
+    def each(call, ok, bad):
+        call(**ok)
+        for name, value, kind, why in bad:
+            with pytest.raises(kind, match=why):
+                call(**dict(ok, **{name: value}))
+
+    shifted = z(8 * 128 + 4)[1:8 * 128 + 1].view(8, 128)                               # rows off their 16-byte boundaries
+    for t in (torch.float32, torch.bfloat16):
+        r = z(8, 512, t=t)
+        other = torch.bfloat16 if t is torch.float32 else torch.float32
+        each(K.attn_prompt, dict(q=r[:, :128], k=r[:, 128:192], v=r[:, 192:256], cu=iz(2), out=z(8, 128, t=t), heads=2, kv_heads=1), [
+            ('q', z(8, 128, t=torch.float16), ValueError, 'q must be fp32 or bf16'), ('k', z(8, 64, t=other), ValueError, 'k must be a 2-D'),
+            ('q', torch.zeros(8, 128, dtype=t), ValueError, 'on the current GPU'), ('q', z(8, 130, t=t), ValueError, 'not a multiple'),
+            ('q', z(8, 2, 64, t=t), ValueError, 'q must be'), ('v', z(7, 64, t=t), ValueError, 'v must hold'), ('k', z(8, 56, t=t), ValueError, 'k must hold'),
+            ('k', z(64, 8, t=t).t(), ValueError, 'inner stride'), ('k', z(1, 64, t=t).expand(8, 64), ValueError, 'overlap'),
+            ('k', z(8, 66, t=t)[:, :64], ValueError, '16 bytes'), ('out', r[:, :128], ValueError, 'out must not overlap'),
+            ('out', r[:, 64:192], ValueError, 'out must not overlap'), ('cu', iz(2).long(), ValueError, 'cu must be'), ('cu', None, TypeError, 'cu must be a tensor'),
+            ('cu', iz(4)[::2], ValueError, 'cu must be'), ('cu', iz(0), ValueError, 'cu must be'), ('heads', 3, ValueError, 'heads'), ('heads', 0, ValueError, 'heads'),
+            ('kv_heads', 0, ValueError, 'heads'), ('heads', 1.5, TypeError, 'heads must be an integer'), ('q', None, TypeError, 'q must be a tensor'),
+            ('q', [1], TypeError, 'q must be a tensor'), ('scale', math.nan, TstError, 'not finite'), ('scale', 'x', TypeError, 'real number|float')])
+    with pytest.raises(ValueError, match='16-byte'):
+        K.attn_prompt(shifted, rows[:, :128], rows[:, 128:], iz(2), z(8, 128), 1)
+    plan = dict(lens=iz(3), room=None, pages=iz(5), page=32, table=iz(3, 4), cu=iz(4), slots=iz(9), pos=iz(9), seq=iz(9), used=iz(1))
+    each(K.page_plan, plan, [
+        ('lens', None, TypeError, 'lens'), ('lens', iz(3, 1), ValueError, 'lens must be'), ('room', iz(2), ValueError, 'room must be'), ('pages', None, TypeError, 'pages'),
+        ('page', 24, TstError, 'power of two'), ('page', 'a', TypeError, 'page must be an integer'), ('table', iz(2, 4), ValueError, 'table must be'),
+        ('table', iz(3, 8)[:, :4], ValueError, 'table must be'), ('cu', iz(3), ValueError, 'cu must be'), ('pos', iz(8), ValueError, 'pos must be'),
+        ('seq', z(9), ValueError, 'seq must be'), ('used', iz(0), ValueError, 'used must be'), ('used', None, TstError, 'null pointer'), ('slots', None, TypeError, 'slots')])
+    each(K.page_step, dict(base=iz(3), sent=None, t=0, table=iz(3, 4), page=32, slots=iz(3), pos=iz(3), lens=iz(3), n_rows=3), [
+        ('base', iz(2), ValueError, 'base must be'), ('sent', iz(2), ValueError, 'sent must be'), ('lens', iz(2), ValueError, 'lens must be'),
+        ('n_rows', -1, TstError, 'negative'), ('t', None, TypeError, 't must be an integer'), ('table', iz(3), ValueError, 'table must be'),
+        ('n_rows', 1 << 70, TypeError, 'integer')])
+    cache = K.Cache4(3, 32, 2, 64)
+    no = iz(8) - 1
+    each(K.cache4_write, dict(cache=cache, k=rows[:, :128], v=rows[:, 128:], slots=no, n_rows=8), [
+        ('k', z(8, 120), ValueError, 'k must hold'), ('v', z(8, 128, t=torch.bfloat16), ValueError, 'v must be a 2-D'), ('slots', no[:7], ValueError, 'slots must be'),
+        ('n_rows', 9, ValueError, 'must hold'), ('k', z(8, 128).double(), ValueError, 'rows must be fp32 or bf16'), ('slots', None, TstError, 'null pointer')])
+    each(K.cache4_read, dict(cache=cache, k=z(8, 128), v=z(8, 128), slots=no, n_rows=8), [
+        ('k', z(8, 120), ValueError, 'k must hold'), ('slots', no.long(), ValueError, 'slots must be'), ('v', shifted, ValueError, '16-byte')])
+    cache.dev += 1                                                                     # as if it were on another device
+    for call, a in ((K.cache4_write, (rows[:, :128], rows[:, 128:], no, 8)), (K.cache4_read, (no, rows[:, :128], rows[:, 128:], 8))):
+        with pytest.raises(ValueError, match='the current device is'):
+            call(cache, *a)
+    cache.dev -= 1
+    each(K.attn_cache4, dict(q=rows, cache=cache, table=iz(8, 3), lens=iz(8), out=z(8, 256), n_rows=8, heads=4, max_len=96), [
+        ('heads', 3, ValueError, 'multiple of the cache'), ('q', rows[:, :248], ValueError, 'q must hold'), ('out', rows, ValueError, 'overlap'),
+        ('table', iz(8), ValueError, 'table must be'), ('seq', iz(7), ValueError, 'seq must be'), ('lens', iz(7), ValueError, 'lens must be'),
+        ('lens', None, TstError, 'null pointer'), ('work', z(9)[1:].double(), ValueError, 'work must be'), ('max_len', -1, ValueError, 'bad sizes'),
+        ('scale', math.inf, TstError, 'not finite')])
+    with pytest.raises(TstError, match='are needed'):
+        K.attn_cache4(rows, cache, iz(8, 300), iz(8), z(8, 256), 8, 4, 9000, work=z(4))
+    x = z(8, 100)
+    full = dict(logits=x, n_rows=8, n_cols=100, out=x, params=z(8, 3), hist=iz(8, 5), hist_len=iz(8), prompt=iz(6), prompt_cu=iz(9), bias=z(1, 100),
+                bias_row=None, mask=iz(2, 4), mask_row=iz(8))
+    each(K.adjust_logits, full, [
+        ('out', z(8, 100, t=torch.bfloat16), ValueError, 'one type'), ('out', z(7, 100), ValueError, 'out must hold'), ('n_cols', 101, ValueError, 'logits must hold'),
+        ('params', z(7, 3), ValueError, 'params must be'), ('params', None, ValueError, 'need params'), ('params', z(8, 4), ValueError, 'params must be'),
+        ('hist', iz(7, 5), ValueError, 'hist must be'), ('hist', iz(5, 8).t(), ValueError, 'hist must be'), ('hist_len', iz(7), ValueError, 'hist_len must be'),
+        ('prompt_cu', None, ValueError, 'needs prompt_cu'), ('prompt_cu', iz(8), ValueError, 'prompt_cu must be'), ('bias', z(1, 99), ValueError, 'bias must be'),
+        ('bias', z(1, 100).half(), ValueError, 'bias must be'), ('mask', iz(2, 3), ValueError, 'mask must be'), ('mask_row', iz(7), ValueError, 'mask_row must be'),
+        ('logits', x.half(), ValueError, 'fp32 or bf16'), ('sent', iz(7), ValueError, 'sent must be')])
+    wide = z(16, 100)
+    with pytest.raises(ValueError, match='out must be logits or not overlap it'):
+        K.adjust_logits(wide[:8], 8, 100, wide[4:12])
+    state = iz(4)
+    each(K.grammar_next, dict(table=iz(2, 7), state=state, parent=None, tok=iz(4), out=iz(4), n_rows=4), [
+        ('out', state, ValueError, 'out must not be state'), ('state', None, TypeError, 'state'), ('tok', iz(3), ValueError, 'tok must be'),
+        ('tok', None, TstError, 'null pointer'), ('table', iz(7), ValueError, 'table must be'), ('parent', iz(3), ValueError, 'parent must be')])
+    torch.cuda.synchronize()

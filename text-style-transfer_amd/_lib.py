@@ -4,6 +4,7 @@ The library is built in-tree by ``csrc/build.sh`` (``__graft_entry__.build()``).
 if it is missing, importing this module raises, and every wrapper raises on a non-zero status.
 """
 import ctypes
+import importlib.util
 import os
 
 # torch must be loaded first: the library's dependency on libamdhip64.so.7 then binds to the HIP runtime
@@ -192,6 +193,19 @@ for _name, (_args, _res) in _PROTOS.items():
 
 class TstError(RuntimeError):
     pass
+
+
+# The prompted-decoding calls are checked and issued by an extension module (csrc/calls.cpp), built by the same script; it calls the
+# entry points of the library loaded above.
+_CALLS_PATH = os.path.join(_HERE, '_tst_calls.so')
+if not os.path.exists(_CALLS_PATH):
+    raise ImportError('%s is missing: build it with text-style-transfer_amd/csrc/build.sh' % _CALLS_PATH)
+_spec = importlib.util.spec_from_file_location('_tst_calls', _CALLS_PATH)
+calls = importlib.util.module_from_spec(_spec)
+_spec.loader.exec_module(calls)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+calls.bind({n: ctypes.cast(getattr(_dll, n), c_vp).value for n in _PROTOS}, getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device),
+           _raw_stream if _raw_stream is not None else lambda dev: torch.cuda.current_stream(dev).cuda_stream, TstError)
 
 
 def call(name, *args):

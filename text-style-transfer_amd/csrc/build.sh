@@ -26,4 +26,13 @@ done
 OBJS=""
 for f in $UNITS; do OBJS="$OBJS $f.o"; done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $OUT $OBJS
+# the checked calls of the prompted-decoding kernels, a host-only extension module
+CALLS=../_tst_calls.so
+if [ ! -f $CALLS ] || [ calls.cpp -nt $CALLS ] || [ build.sh -nt $CALLS ] || [ ../../include/tst_hip.h -nt $CALLS ]; then
+  rm -f $CALLS
+  TORCH=$(python3 -c "import importlib.util as u; print(u.find_spec('torch').submodule_search_locations[0])")
+  PY=$(python3 -c "import sysconfig; print(sysconfig.get_path('include'))")
+  g++ -O2 -std=c++17 -fPIC -shared -fvisibility=hidden -Wall -D_GLIBCXX_USE_CXX11_ABI=1 -I../../include -I$PY -I$TORCH/include \
+    -I$TORCH/include/torch/csrc/api/include calls.cpp -o $CALLS -L$TORCH/lib -ltorch_python -ltorch_cpu -lc10
+fi
 echo "built $OUT"

@@ -630,81 +630,16 @@ def retire_compact(cur, nxt, sel, lp, n_sent, k, step, T, eos, last_step, top_en
 
 # ---- prompted decoding: packed prompts, pages, a cache in 4 bits, rules on logits --------------------------------------------------
 
-_I32, _U8, _F32, _BF16 = torch.int32, torch.uint8, torch.float32, torch.bfloat16
-_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)
-_stream_of = _raw_stream if _raw_stream is not None else lambda dev: torch.cuda.current_stream(dev).cuda_stream
-
-
-# The checks below run on every call of kernels that take a few microseconds: each asks a tensor for as little as it can.  All tensors
-# have to live on the current device, on whose current stream the kernels run (``dev``: its number; a CPU tensor answers -1).
-
-def _rows2d(t, dtype, dev, n_rows, n_cols, name):
-    """(address, leading dimension) of a 2-D view whose rows the kernels can read 16 bytes at a time."""
-    shape, stride = t.shape, t.stride()
-    if t.dtype is not dtype or len(shape) != 2 or t.get_device() != dev or (stride[1] != 1 and shape[1] > 1):
-        raise ValueError('%s must be a 2-D %s tensor with unit inner stride on the current GPU, got %s %s on %s'
-                         % (name, dtype, t.dtype, tuple(shape), t.device))
-    if shape[0] < n_rows or shape[1] < n_cols:
-        raise ValueError('%s must hold [%d, %d], got %s' % (name, n_rows, n_cols, tuple(shape)))
-    unit = 4 if dtype is _F32 else 8
-    ld = stride[0]
-    if n_rows <= 1:
-        ld = max(ld, n_cols)
-        ld += -ld % unit
-    elif ld < n_cols or ld % unit:
-        raise ValueError('rows of %s must not overlap and start at multiples of %d elements (16 bytes)' % (name, unit))
-    at = t.data_ptr()
-    if at & 15:
-        raise ValueError('%s must start at a 16-byte boundary' % name)
-    return at, ld
-
-
-def _ints(t, n, dev, name):
-    """Address of a 1-D int32 tensor of at least n entries (None: a null pointer)."""
-    if t is None:
-        return None
-    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
-        raise ValueError('%s must be a contiguous int32 tensor [%d] on the current GPU, got %s %s on %s' % (name, n, t.dtype, tuple(t.shape), t.device))
-    return t.data_ptr()
-
-
-def _table(t, dev, name):
-    shape = t.shape
-    if t.dtype is not _I32 or len(shape) != 2 or t.get_device() != dev or not t.is_contiguous():
-        raise ValueError('%s must be a contiguous 2-D int32 tensor on the current GPU, got %s %s on %s' % (name, t.dtype, tuple(shape), t.device))
-    return shape
-
-
-def _disjoint(a, lda, b, ldb, n_rows, cols_a, cols_b, size, what):
-    """Raises if the first n_rows rows of two views (addresses, leading dimensions, widths, element size) share a byte's range."""
-    if n_rows > 0 and a < b + ((n_rows - 1) * ldb + cols_b) * size and b < a + ((n_rows - 1) * lda + cols_a) * size:
-        raise ValueError(what)
+# These kernels take a few microseconds: their arguments are checked natively (csrc/calls.cpp, ValueError and TypeError like everywhere).
+# All tensors have to live on the current device, on whose current stream the kernels run.
+_calls = _lib.calls
 
 
 def attn_prompt(q, k, v, cu, out, heads, kv_heads=None, scale=None):
     """Causal attention over packed prompts: rows cu[b] .. cu[b + 1] - 1 of q [N, heads * dh], k, v [N, kv_heads * dh] (views with
     unit inner stride, fp32 or bf16) are sequence b; head h reads key head h // (heads / kv_heads).  ``out`` [N, heads * dh] must not
     overlap them; its rows outside every sequence are left alone.  ``scale``: 1 / sqrt(dh) unless given."""
-    if kv_heads is None:
-        kv_heads = heads
-    dt, dev = q.dtype, _device()
-    if dt is not _BF16 and dt is not _F32:
-        raise ValueError('q must be fp32 or bf16')
-    if q.dim() != 2 or heads < 1 or kv_heads < 1 or heads % kv_heads or q.shape[1] % heads:
-        raise ValueError('q must be [tokens, heads * head size], heads a multiple of kv_heads')
-    N, wq = q.shape
-    dh = wq // heads
-    unit, size = (8, 2) if dt is _BF16 else (4, 4)
-    if dh % unit or not 0 < dh <= 256:
-        raise ValueError('head size %d is not a multiple of %d up to 256' % (dh, unit))
-    wk = kv_heads * dh
-    (pq, ldq), (pk, ldk) = _rows2d(q, dt, dev, N, wq, 'q'), _rows2d(k, dt, dev, N, wk, 'k')
-    (pv, ldv), (po, ldo) = _rows2d(v, dt, dev, N, wk, 'v'), _rows2d(out, dt, dev, N, wq, 'out')
-    pc = _ints(cu, 1, dev, 'cu')
-    for p, ld, w in ((pq, ldq, wq), (pk, ldk, wk), (pv, ldv, wk)):
-        _disjoint(po, ldo, p, ld, N, wq, w, size, 'out must not overlap q, k or v')
-    call('tst_attn_prompt_bf16' if dt is _BF16 else 'tst_attn_prompt_f32', pq, ldq, pk, ldk, pv, ldv, pc, cu.numel() - 1, po, ldo, N, heads, kv_heads,
-         dh, dh ** -0.5 if scale is None else scale, _stream_of(dev))
+    _calls.attn_prompt(q, k, v, cu, out, heads, kv_heads, scale)
 
 
 def page_plan(lens, room, pages, page, table, cu, slots, pos, seq, used):
@@ -712,25 +647,13 @@ def page_plan(lens, room, pages, page, table, cu, slots, pos, seq, used):
     ``pages`` in order.  Writes ``table`` [B, width] (-1 where there is no page), ``cu`` [B + 1], and per packed token ``slots``,
     ``pos``, ``seq`` (entries behind the last token stay as they are); ``used`` [1] = pages needed, more than ``pages`` holds if
     the list is too short (the entries that got none are -1).  All int32; ``page`` a power of two in 8 .. 1024."""
-    dev = _device()
-    B, N, n_pages = lens.numel(), slots.numel(), pages.numel()
-    rows, width = _table(table, dev, 'table')
-    if rows != B:
-        raise ValueError('table must be [sequences, width]')
-    if n_pages * page > 0x7fffffff:
-        raise ValueError('pages * page exceeds 2^31 - 1: slots are 32-bit')
-    call('tst_page_plan', _ints(lens, B, dev, 'lens'), _ints(room, B, dev, 'room'), B, _ints(pages, 0, dev, 'pages'), n_pages, page, table.data_ptr(),
-         width, _ints(cu, B + 1, dev, 'cu'), _ints(slots, N, dev, 'slots'), _ints(pos, N, dev, 'pos'), _ints(seq, N, dev, 'seq'), N,
-         _ints(used, 1, dev, 'used'), _stream_of(dev))
+    _calls.page_plan(lens, room, pages, page, table, cu, slots, pos, seq, used)
 
 
 def page_step(base, sent, t, table, page, slots, pos, lens, n_rows):
     """Step ``t`` of decoding over a page table: row r continues sequence ``sent[r]`` (None: r) at position base + t: ``pos``, ``lens``
     (= pos + 1) and ``slots`` (-1 without a page) of the first ``n_rows`` rows."""
-    dev = _device()
-    n_seq, width = _table(table, dev, 'table')
-    call('tst_page_step', _ints(base, n_seq, dev, 'base'), _ints(sent, n_rows, dev, 'sent'), t, table.data_ptr(), width, n_seq, page,
-         _ints(slots, n_rows, dev, 'slots'), _ints(pos, n_rows, dev, 'pos'), _ints(lens, n_rows, dev, 'lens'), n_rows, _stream_of(dev))
+    _calls.page_step(base, sent, t, table, page, slots, pos, lens, n_rows)
 
 
 class Cache4:
@@ -751,37 +674,25 @@ class Cache4:
         if tensors is None:
             tensors = [torch.zeros(s, dtype=torch.uint8, device=device) for s in shapes]
         for t, s, nm in zip(tensors, shapes, ('kc', 'ks', 'vc', 'vs')):
-            if not (t.is_cuda and t.device == tensors[0].device and t.dtype is _U8 and tuple(t.shape) == s and t.is_contiguous()
+            if not (t.is_cuda and t.device == tensors[0].device and t.dtype is torch.uint8 and tuple(t.shape) == s and t.is_contiguous()
                     and t.data_ptr() % 16 == 0):
                 raise ValueError('%s must be a contiguous, 16-byte aligned uint8 tensor %s on the GPU' % (nm, list(s)))
         self.kc, self.ks, self.vc, self.vs = tensors
         self.dev = tensors[0].get_device()
         self.c = _lib.TstCache4(kc=_p(self.kc), ks=_p(self.ks), vc=_p(self.vc), vs=_p(self.vs), pages=pages, page=page, kv_heads=kv_heads,
                                 dh=head_size, reserved=0)
-
-    def _on(self, dev):
-        if self.dev != dev:
-            raise ValueError('the cache is on cuda:%d, the current device is cuda:%d' % (self.dev, dev))
-        return self.c
+        self._at = _lib.ctypes.addressof(self.c)
 
 
 def cache4_write(cache, k, v, slots, n_rows):
     """Rows 0 .. n_rows - 1 of k and v ([n, kv_heads * dh], fp32 or bf16) into the cache at ``slots`` (page * page size + token; a
     slot outside the cache stores nothing; no slot twice)."""
-    dt, w, dev = k.dtype, cache.kv_heads * cache.dh, _device()
-    if dt is not _BF16 and dt is not _F32:
-        raise ValueError('rows must be fp32 or bf16')
-    call('tst_cache4_write_bf16' if dt is _BF16 else 'tst_cache4_write_f32', cache._on(dev), *_rows2d(k, dt, dev, n_rows, w, 'k'),
-         *_rows2d(v, dt, dev, n_rows, w, 'v'), _ints(slots, n_rows, dev, 'slots'), n_rows, _stream_of(dev))
+    _calls.cache4_write(cache._at, cache.dev, k, v, slots, n_rows)
 
 
 def cache4_read(cache, slots, k, v, n_rows):
     """The rows at ``slots`` as the values their codes stand for (zeros for a slot outside the cache); k and v must not overlap."""
-    dt, w, dev = k.dtype, cache.kv_heads * cache.dh, _device()
-    if dt is not _BF16 and dt is not _F32:
-        raise ValueError('rows must be fp32 or bf16')
-    call('tst_cache4_read_bf16' if dt is _BF16 else 'tst_cache4_read_f32', cache._on(dev), _ints(slots, n_rows, dev, 'slots'),
-         *_rows2d(k, dt, dev, n_rows, w, 'k'), *_rows2d(v, dt, dev, n_rows, w, 'v'), n_rows, _stream_of(dev))
+    _calls.cache4_read(cache._at, cache.dev, slots, k, v, n_rows)
 
 
 def attn_cache4_work(n_rows, heads, kv_heads, head_size, max_len, device='cuda'):
@@ -797,31 +708,9 @@ def attn_cache4(q, cache, table, lens, out, n_rows, heads, max_len, seq=None, sc
     """One step's attention over a 4-bit cache: row r of q [n_rows, heads * dh] (fp32 or bf16) attends to the first ``lens[r]`` tokens
     of sequence ``seq[r]`` (None: r) of the page table.  No token to attend to gives zeros.  ``max_len``: an upper bound of
     ``lens`` (longer rows are cut to it).  ``work``: scratch of ``attn_cache4_work``, made here when None."""
-    dt, dh, dev = q.dtype, cache.dh, _device()
-    if dt is not _BF16 and dt is not _F32:
-        raise ValueError('q must be fp32 or bf16')
-    if heads < 1 or heads % cache.kv_heads:
-        raise ValueError("heads must be a multiple of the cache's %d" % cache.kv_heads)
-    w = heads * dh
-    (pq, ldq), (po, ldo) = _rows2d(q, dt, dev, n_rows, w, 'q'), _rows2d(out, dt, dev, n_rows, w, 'out')
-    _disjoint(po, ldo, pq, ldq, n_rows, w, w, 2 if dt is _BF16 else 4, 'out must not overlap q')
-    n_seq, width = _table(table, dev, 'table')
-    if work is None:
-        work = attn_cache4_work(n_rows, heads, cache.kv_heads, dh, max_len, q.device)
-    elif work.dtype is not _F32 or work.get_device() != dev or not work.is_contiguous():
-        raise ValueError('work must be a contiguous fp32 tensor on the current GPU')
-    call('tst_attn_cache4_bf16' if dt is _BF16 else 'tst_attn_cache4_f32', cache._on(dev), pq, ldq, table.data_ptr(), width, n_seq,
-         _ints(seq, n_rows, dev, 'seq'), _ints(lens, n_rows, dev, 'lens'), max_len, po, ldo, n_rows, heads, dh ** -0.5 if scale is None else scale,
-         None if work is None else work.data_ptr(), 0 if work is None else work.numel(), _stream_of(dev))
-
-
-def _rule_rows(t, dtype, width, dev, name):
-    """(address, leading dimension, rows) of a bias or mask table."""
-    shape, stride = t.shape, t.stride()
-    if (t.dtype is not dtype or len(shape) != 2 or t.get_device() != dev or shape[1] < width or (stride[1] != 1 and shape[1] > 1)
-            or (shape[0] > 1 and stride[0] < width)):
-        raise ValueError('%s must be a 2-D %s tensor [n, %d] with unit inner stride on the current GPU' % (name, dtype, width))
-    return t.data_ptr(), max(stride[0], width), shape[0]
+    if work is None and heads > 0 and heads % cache.kv_heads == 0:
+        work = attn_cache4_work(n_rows, heads, cache.kv_heads, cache.dh, max_len, q.device)
+    _calls.attn_cache4(cache._at, cache.dev, q, table, lens, out, n_rows, heads, max_len, seq, scale, work)
 
 
 def adjust_logits(logits, n_rows, n_cols, out, *, params=None, sent=None, hist=None, hist_len=None, prompt=None, prompt_cu=None, bias=None,
@@ -831,60 +720,12 @@ def adjust_logits(logits, n_rows, n_cols, out, *, params=None, sent=None, hist=N
     or per row), ``bias`` [n, >= V] fp32, ``mask`` [n, >= ceil(V / 32)] int32 words (bit 0 = forbidden = -inf).  ``hist`` [rows, n]
     int32 tokens with ``hist_len`` [rows] valid ones (None: all); ``prompt`` packed int32 tokens with offsets ``prompt_cu`` [n + 1];
     ``bias_row`` / ``mask_row`` [rows] choose a row (None: row 0, -1: none).  ``out`` may be ``logits``.  fp32 or bf16."""
-    dev, dt = _device(), logits.dtype
-    if dt is not _F32 and dt is not _BF16:
-        raise ValueError('logits must be fp32 or bf16')
-    lds = []
-    for t, nm in ((logits, 'logits'), (out, 'out')):
-        shape, stride = t.shape, t.stride()
-        if t.dtype is not dt or len(shape) != 2 or t.get_device() != dev or (stride[1] != 1 and shape[1] > 1):
-            raise ValueError('logits and out must be 2-D tensors of one type with unit inner stride on the current GPU')
-        if shape[0] < n_rows or shape[1] < n_cols or (n_rows > 1 and stride[0] < n_cols):
-            raise ValueError('%s must hold [%d, %d] without overlapping rows' % (nm, n_rows, n_cols))
-        lds.append(max(stride[0], n_cols))
-    p_in, p_out = logits.data_ptr(), out.data_ptr()
-    if p_in != p_out:
-        _disjoint(p_out, lds[1], p_in, lds[0], n_rows, n_cols, n_cols, 4 if dt is _F32 else 2, 'out must be logits or not overlap it')
-    rules = _lib.TstLogitRules()
-    if params is not None:
-        if (params.dtype is not _F32 or params.dim() != 2 or params.shape[1] != 3 or params.get_device() != dev or not params.is_contiguous()
-                or (sent is None and params.shape[0] < n_rows)):
-            raise ValueError('params must be a contiguous fp32 tensor [sentences, 3] on the current GPU')
-        rules.params, rules.n_sent = params.data_ptr(), params.shape[0]
-    elif hist is not None or prompt is not None:
-        raise ValueError('hist and prompt need params')
-    if sent is not None:
-        rules.sent = _ints(sent, n_rows, dev, 'sent')
-    if hist is not None:
-        shape, stride = hist.shape, hist.stride()
-        if (hist.dtype is not _I32 or len(shape) != 2 or hist.get_device() != dev or shape[0] < n_rows or (stride[1] != 1 and shape[1] > 1)
-                or (n_rows > 1 and stride[0] < shape[1])):
-            raise ValueError('hist must be int32 [rows, tokens] with unit inner stride on the current GPU')
-        rules.hist, rules.ld_hist, rules.n_hist = hist.data_ptr(), max(stride[0], shape[1]), shape[1]
-        rules.hist_len = _ints(hist_len, n_rows, dev, 'hist_len')
-    if prompt is not None:
-        if prompt_cu is None:
-            raise ValueError('prompt needs prompt_cu')
-        rules.prompt, rules.n_prompt = _ints(prompt, 0, dev, 'prompt'), prompt.numel()
-        rules.prompt_cu = _ints(prompt_cu, rules.n_sent + 1, dev, 'prompt_cu')
-    if bias is not None:
-        rules.bias, rules.ld_bias, rules.n_bias = _rule_rows(bias, _F32, n_cols, dev, 'bias')
-        rules.bias_row = _ints(bias_row, n_rows, dev, 'bias_row')
-    if mask is not None:
-        rules.mask, rules.ld_mask, rules.n_masks = _rule_rows(mask, _I32, (n_cols + 31) // 32, dev, 'mask')
-        rules.mask_row = _ints(mask_row, n_rows, dev, 'mask_row')
-    call('tst_adjust_logits_bf16' if dt is _BF16 else 'tst_adjust_logits_f32', p_in, lds[0], n_rows, n_cols, rules, p_out, lds[1], _stream_of(dev))
+    _calls.adjust_logits(logits, n_rows, n_cols, out, params, sent, hist, hist_len, prompt, prompt_cu, bias, bias_row, mask, mask_row)
 
 
 def grammar_next(table, state, parent, tok, out, n_rows):
     """out[r] = table[state[parent[r]], tok[r]] (``parent`` None: r); -1 stays -1 and is what leaves the table."""
-    dev = _device()
-    n_states, V = _table(table, dev, 'table')
-    ps, po = _ints(state, 0, dev, 'state'), _ints(out, n_rows, dev, 'out')
-    if po == ps:
-        raise ValueError('out must not be state')
-    call('tst_grammar_next', table.data_ptr(), n_states, V, ps, state.numel(), _ints(parent, n_rows, dev, 'parent'), _ints(tok, n_rows, dev, 'tok'), po, n_rows,
-         _stream_of(dev))
+    _calls.grammar_next(table, state, parent, tok, out, n_rows)
 
 
 class PagedPlan:
