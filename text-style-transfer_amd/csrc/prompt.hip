@@ -18,7 +18,7 @@
 // wave per SIMD) 532 us; products of one tile between the exponentials of the one before 562 us; fragments requested where they are used
 // 502 us, 4 keys' and 2 values' products ahead 495 us; of 499 us, 29 were the softmax's arithmetic and 126 waiting for LDS.
 // 256 prompts of 1 .. 512 tokens, 8 heads of 64: 78 us, 3.4 TB/s, half of it waiting: a workgroup has few tiles, and nearly all of them pass
-// the diagonal.  In fp32, 16 prompts of 1 .. 60 tokens, 2 heads of 128: 12.9 us (a tile of 32 keys 3.8 us, a third of it its products); 8
+// the diagonal.  In fp32, 16 prompts of 1 .. 60 tokens, 2 heads of 128: 12.7 us (a tile of 32 keys 3.7 us, a third of it its products); 8
 // prompts of 2048, 8 heads of 64: 134 TFLOP/s.
 //
 // fp32 inputs are split into three bf16 pieces (8 + 8 + 8 bits of significand, exactly the fp32 value) when a tile is staged, and the six
@@ -159,8 +159,8 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
     constexpr int BUF = 2 * NP * PLANE;              // K pieces, then V pieces
     constexpr int KS = DH / 16, MT = DH / 32, NS = KT / 32;
     constexpr int PER = KT * CH / 256;               // chunks of K (and of V) that a thread stages
-    constexpr bool AHEAD = DMA && DH <= 128;         // fragments are requested KD (VD) products before they are wanted
-    constexpr int KD = AHEAD ? 4 : 1, VD = AHEAD ? 2 : 1;
+    constexpr bool AHEAD = (DMA || NP == 3) && DH <= 128;         // fragments are requested KD (VD) products before they are wanted
+    constexpr int KD = AHEAD ? (NP == 3 ? 2 : 4) : 1, VD = AHEAD ? 2 : 1;
     __shared__ __attribute__((aligned(16))) unsigned char smem[(DMA ? 2 : 1) * BUF];
 
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
