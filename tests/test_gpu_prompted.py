@@ -194,6 +194,40 @@ def test_prompt_scores_that_outgrow_the_first_tiles(K, dh, growth, size, dtype):
     check_prompt(q, k, v, [0, L], out, heads, heads, dh, dtype, scale=1.0)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('heads,kv_heads,dh', [(4, 2, 32), (4, 4, 64), (8, 2, 128), (2, 1, 256)])
+def test_prompt_short_alone_and_beside_a_long_one(K, heads, kv_heads, dh, dtype):
+    """Short prompts among themselves (rows spread differently over the GPU) and in front of a long one: right, and the same bits."""
+    short = [20, 33, 1, 0, 64, 7, 100, 32, 65, 2]
+    q, k, v, cu, out = prompt_case(K, short + [900], heads, kv_heads, dh, dtype, seed=dh)
+    check_prompt(q, k, v, cu, out, heads, kv_heads, dh, dtype)
+    n = cu[len(short)]
+    alone = torch.empty_like(out[:n])
+    K.attn_prompt(q[:n], k[:n], v[:n], i32(cu[:len(short) + 1]), alone, heads, kv_heads)
+    assert torch.equal(alone, out[:n])
+
+
+@pytest.mark.parametrize('B', [63, 64, 65, 130, 4097])
+def test_prompt_many_sequences(K, B):
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 5, (B,), generator=g).tolist()
+    lens[0], lens[B // 2], lens[-1] = 3, 40, 2
+    q, k, v, cu, out = prompt_case(K, lens, 2, 1, 32, torch.bfloat16, seed=B, behind=3)
+    assert (out[cu[-1]:] == 7).all()
+    rows = torch.arange(cu[-1], device='cuda')
+    start = torch.repeat_interleave(torch.tensor(cu[:-1], device='cuda'), torch.tensor(lens, device='cuda'))
+    live = (rows.unsqueeze(0) <= rows.unsqueeze(1)) & (rows.unsqueeze(0) >= start.unsqueeze(1))
+    for h in range(2):
+        qd, kd, vd = q[:cu[-1], 32 * h:32 * h + 32].double(), k[:cu[-1]].double(), v[:cu[-1]].double()
+        s = (qd @ kd.t()) * 32 ** -0.5
+        mag = (qd.abs() @ kd.abs().t()) * 32 ** -0.5
+        s, mag = s.masked_fill(~live, -math.inf), mag.masked_fill(~live, 0.0)
+        w = torch.softmax(s, 1)
+        wide = torch.where(w > 1e-12, s.amax(1, keepdim=True) - s, torch.zeros_like(s)).amax(1, keepdim=True)
+        rel = 2 * (2 * (32 * 3 + 2) * U32 * mag.amax(1, keepdim=True) + (4 * wide + 4 + 2 * 40) * U32)
+        check(out[:cu[-1], 32 * h:32 * h + 32], w @ vd, w @ vd.abs(), rel, True)
+
+
 def test_prompt_offsets_beyond_32_bits(K):
     buf = torch.empty((33000, 1 << 16), device='cuda', dtype=torch.bfloat16)     # 4.3 GB, 2.16e9 elements
     cu = [32770, 33000]

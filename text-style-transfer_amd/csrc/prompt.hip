@@ -150,18 +150,19 @@ __device__ __forceinline__ void one_row(const PromptArgs& a, int64_t c0, int64_t
 }
 
 // DMA: bf16 rows of exactly DH elements go from memory to LDS without registers, two buffers; else through registers, one buffer.
-template <typename T, int DH, int KT, bool DMA>
-__global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_kernel(PromptArgs a) {
-    constexpr int BM = 128;                          // rows per workgroup, 32 to a wave
+template <typename T, int DH, int KT, bool DMA, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_prompt_kernel(PromptArgs a) {
+    constexpr int NT = 64 * WAVES, BM = 32 * WAVES;  // threads, rows per workgroup
     constexpr int NP = sizeof(T) == 4 ? 3 : 1;
     constexpr int CH = DH / 8;                       // chunks per row of a tile
     constexpr int PLANE = KT * DH * 2;               // bytes of one piece of a tile
     constexpr int BUF = 2 * NP * PLANE;              // K pieces, then V pieces
     constexpr int KS = DH / 16, MT = DH / 32, NS = KT / 32;
-    constexpr int PER = KT * CH / 256;               // chunks of K (and of V) that a thread stages
+    constexpr int PER = KT * CH / NT;                // chunks of K (and of V) that a thread stages
     constexpr bool AHEAD = (DMA || NP == 3) && DH <= 128;         // fragments are requested KD (VD) products before they are wanted
     constexpr int KD = AHEAD ? (NP == 3 ? 2 : 4) : 1, VD = AHEAD ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[(DMA ? 2 : 1) * BUF];
+    constexpr bool DOUBLE = DMA && WAVES > 1;        // two tiles in LDS: the next one lands while this one is worked on
+    __shared__ __attribute__((aligned(16))) unsigned char smem[(DOUBLE ? 2 : 1) * BUF];
 
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int col = lane & 31, h = lane >> 5;
@@ -176,7 +177,8 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
         const uint32_t xcd = id & 7u;
         id >>= 3;
         head = (int)(id % (uint32_t)a.heads);
-        id = id / (uint32_t)a.heads * 8u + xcd;
+        id /= (uint32_t)a.heads;
+        id = id * 8u + ((xcd + 3u * id) & 7u);   // rotated, so that tiles without rows, every second or third for some lengths, meet every XCD
         if (id >= (uint32_t)a.tiles) return;
     } else {
         const int key_head = (int)(id % (uint32_t)a.kv_heads);
@@ -186,17 +188,23 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
     }
     const int g = head / a.per_kv;
     id = (uint32_t)a.tiles - 1u - id;
-    // Sequence b owns tile numbers from cu[b] / BM + b on: strictly ascending, and always enough of them
-    // (a search by 64 probes at once: two dependent loads for 4096 sequences instead of twelve)
-    int lo = 0;
-    for (int n = a.B; n > 1;) {
+    // Sequence b owns tile numbers from cu[b] / BM + b on: strictly ascending, and always enough of them.  A search by 64 probes at once, the
+    // last of which also hold the sequence's ends: one load for up to 64 sequences, two for 4096.
+    int lo = 0, begin, end;
+    for (int n = a.B;;) {
         const int step = (n + 63) >> 6, at = lo + lane * step;
-        const bool starts = lane * step < n && (int64_t)(a.cu[at] / BM) + at <= (int64_t)id;
+        const int probe = lane * step <= n ? a.cu[at] : 0;
+        const bool starts = lane * step < n && (int64_t)(probe / BM) + at <= (int64_t)id;
         const int count = max(__builtin_popcountll(__ballot(starts)), 1) - 1;
         lo += count * step;
+        if (step == 1) {
+            begin = __builtin_amdgcn_readlane(probe, count);
+            end = count < 63 ? __builtin_amdgcn_readlane(probe, count + 1) : a.cu[lo + 1];
+            break;
+        }
         n = min(step, n - count * step);
     }
-    const int64_t c0 = a.cu[lo], c1 = a.cu[lo + 1];
+    const int64_t c0 = begin, c1 = end;
     const int64_t qt = (int64_t)id - (c0 / BM + lo);
     if (c0 < 0 || c1 > a.N || qt < 0 || qt * BM >= c1 - c0) return;      // the whole workgroup
     const int len = (int)(c1 - c0);
@@ -232,7 +240,7 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
 
-    // staging: chunk number x = thread + 256 j of a tile is row x / CH, place x % CH
+    // staging: chunk number x = thread + NT j of a tile is row x / CH, place x % CH
     u32x4 stage_k[DMA ? 1 : PER], stage_v[DMA ? 1 : PER];
     float4 stage_k2[NP == 3 ? PER : 1], stage_v2[NP == 3 ? PER : 1];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
@@ -241,7 +249,7 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
     uint32_t off_k[PER], off_v[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const int x = threadIdx.x + 256 * j, r = x / CH, c = x % CH;
+        const int x = threadIdx.x + NT * j, r = x / CH, c = x % CH;
         off_k[j] = (uint32_t)(r * (int)a.ldk + 8 * (DMA ? c ^ k_swizzle<DH>(r) : c)) * (uint32_t)sizeof(T);
         off_v[j] = (uint32_t)(r * (int)a.ldv + 8 * (DMA ? c ^ v_swizzle<DH>(r) : c)) * (uint32_t)sizeof(T);
     }
@@ -251,7 +259,7 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
         const bool whole = k0 + KT <= len;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int x = threadIdx.x + 256 * j, r = x / CH, c = x % CH;
+            const int x = threadIdx.x + NT * j, r = x / CH, c = x % CH;
             uint32_t ok = off_k[j], ov = off_v[j];
             if (!whole) {                                                // rows behind the sequence: its last one, weighted 0
                 const int back = max(k0 + r - (len - 1), 0);
@@ -259,7 +267,7 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
                 ov -= (uint32_t)(back * (int)a.ldv) * (uint32_t)sizeof(T);
             }
             if (DMA) {
-                const uint32_t dst = lds0 + buf * BUF + (wu * 64 + 256 * j) * 16;
+                const uint32_t dst = lds0 + buf * BUF + (wu * 64 + NT * j) * 16;
                 dma16(dst, tk, ok);
                 dma16(dst + PLANE, tv, ov);
             } else {
@@ -279,7 +287,7 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
     auto put = [&]() {   // registers -> LDS (not used with DMA)
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int x = threadIdx.x + 256 * j, r = x / CH, c = x % CH;
+            const int x = threadIdx.x + NT * j, r = x / CH, c = x % CH;
             unsigned char* dk = smem + r * DH * 2 + (c ^ k_swizzle<DH>(r)) * 16;
             unsigned char* dv = smem + NP * PLANE + r * DH * 2 + (c ^ v_swizzle<DH>(r)) * 16;
             if (NP == 1) {
@@ -320,7 +328,7 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
         if (DMA) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // this tile has landed (this wave's share)
             __syncthreads();                                             // everybody's share; and nobody reads the other buffer any more
-            if (k0 + KT <= q_end) fetch(k0 + KT, buf ^ 1);
+            if (DOUBLE && k0 + KT <= q_end) fetch(k0 + KT, buf ^ 1);
         } else {
             __syncthreads();
             put();
@@ -329,7 +337,7 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
         }
         const unsigned char* kt = smem + buf * BUF;
         const unsigned char* vt = kt + NP * PLANE;
-        if (DMA) buf ^= 1;
+        if (DOUBLE) buf ^= 1;
         if (k0 > w_end || qw >= len) continue;                           // nothing for this wave in the tile
         // EDGE: the wave's first tile (which sets the reference point) and tiles that end behind some row of it
         auto tile = [&](auto edge) {
@@ -447,6 +455,7 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
         };
         if (k0 == 0 || k0 + KT - 1 > qw) tile(std::true_type{});
         else tile(std::false_type{});
+        if (DMA && !DOUBLE && k0 + KT <= q_end) fetch(k0 + KT, 0);            // the wave has used all it read
         // The reference point moves when a sum has outgrown it by 2^60: far from any limit of fp32, and rare.  (A single tile that outgrows it by
         // 2^127 overflows; its rows are computed again at the end.)
         if (__ballot(sum > 0x1p60f) != 0ull) {
@@ -496,20 +505,29 @@ __global__ __launch_bounds__(256, DMA && DH <= 128 ? 2 : 1) void attn_prompt_ker
         one_row<T>(a, c0, c0 + qw + __builtin_ctz(cols), head, g);
 }
 
-template <typename T, int DH, int KT, bool DMA>
+template <typename T, int DH, int KT, bool DMA, int WAVES = 4>
 int launch_one(PromptArgs a, hipStream_t st, const char* who) {
-    const int64_t tiles = a.N / 128 + a.B;                                  // sequence b owns tiles cu[b] / 128 + b ..
+    constexpr int BM = 32 * WAVES;
+    const int64_t tiles = a.N / BM + a.B;                                   // sequence b owns tiles cu[b] / BM + b ..
     a.by_rows = a.N / a.B * a.kv_heads * a.dh * 2 * (int64_t)sizeof(T) <= (1 << 21);
     const int64_t groups = (a.by_rows ? (tiles + 7) / 8 * 8 : tiles) * a.heads;
     TST_REQUIRE(groups <= (int64_t)0x7fffffff, TST_ERR_UNSUPPORTED, "%s: too many row tiles", who);
     a.tiles = (int)tiles;
-    attn_prompt_kernel<T, DH, KT, DMA><<<(unsigned)groups, 256, 0, st>>>(a);
+    attn_prompt_kernel<T, DH, KT, DMA, WAVES><<<(unsigned)groups, 64 * WAVES, 0, st>>>(a);
     return tst_after_launch(who);
 }
 
 template <typename T>
 int launch_prompt(const PromptArgs& a, hipStream_t st, const char* who) {
     if constexpr (sizeof(T) == 2) {
+        // Prompts of a few rows: one wave per workgroup, one tile of 32 keys in LDS, so that many are at work (256 prompts, 32 heads over 8 of
+        // 128: 2 tokens each 19 us, 62 with four waves; 32 tokens 33 and 76; 48 tokens 57 and 90; 96 tokens 142 and 158, but of 8 heads of 64
+        // 27 and 23).  A row's sums run over the same keys in the same order either way.
+        if (a.N / a.B <= 48) {
+            if (a.dh == 32) return launch_one<T, 32, 32, true, 1>(a, st, who);
+            if (a.dh == 64) return launch_one<T, 64, 32, true, 1>(a, st, who);
+            if (a.dh == 128) return launch_one<T, 128, 32, true, 1>(a, st, who);
+        }
         if (a.dh == 32) return launch_one<T, 32, 64, true>(a, st, who);
         if (a.dh == 64) return launch_one<T, 64, 64, true>(a, st, who);
         if (a.dh == 128) return launch_one<T, 128, 64, true>(a, st, who);
@@ -518,6 +536,7 @@ int launch_prompt(const PromptArgs& a, hipStream_t st, const char* who) {
         if (a.dh < 128) return launch_one<T, 128, 64, false>(a, st, who);
         return launch_one<T, 256, 32, false>(a, st, who);
     } else {
+        if (a.dh <= 32) return launch_one<T, 32, 64, false>(a, st, who);
         if (a.dh <= 64) return launch_one<T, 64, 32, false>(a, st, who);
         if (a.dh <= 128) return launch_one<T, 128, 32, false>(a, st, who);
         return launch_one<T, 256, 32, false>(a, st, who);
