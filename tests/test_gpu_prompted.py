@@ -207,6 +207,21 @@ def test_prompt_short_alone_and_beside_a_long_one(K, heads, kv_heads, dh, dtype)
     assert torch.equal(alone, out[:n])
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('heads,kv_heads,dh', [(8, 4, 32), (8, 8, 24), (8, 2, 64), (16, 4, 128), (8, 1, 72)])
+def test_prompt_many_short(K, heads, kv_heads, dh, dtype):
+    """Enough short prompts to fill the GPU several times; some longer than a tile, some empty."""
+    lens = ([3, 17, 0, 32, 33, 1, 66, 8] * 17)[:130]
+    q, k, v, cu, out = prompt_case(K, lens, heads, kv_heads, dh, dtype, seed=dh, before=2, behind=2)
+    first = 8
+    check_prompt(q, k, v, cu[:first + 1], out, heads, kv_heads, dh, dtype)
+    for b in range(first, len(lens), first):                 # the rest against calls of eight at a time: the same bits
+        e = min(b + first, len(lens))
+        part = out.clone()
+        K.attn_prompt(q, k, v, i32(cu[b:e + 1]), part, heads, kv_heads)
+        assert torch.equal(part, out)
+
+
 @pytest.mark.parametrize('B', [63, 64, 65, 130, 4097])
 def test_prompt_many_sequences(K, B):
     g = torch.Generator().manual_seed(B)

@@ -1,6 +1,6 @@
 // Causal attention over whole prompts of different lengths, packed one behind the other, with grouped heads.
 //
-// A workgroup of four waves takes 128 query rows of one sequence and one head, 32 to a wave, and walks the keys in tiles of KT that all
+// A workgroup of four waves (one, for short prompts) takes 128 (32) query rows of one sequence and one head, 32 to a wave, and walks the keys in tiles of KT that all
 // four waves read from LDS.  On v_mfma_f32_32x32x16_bf16:
 //     S^T [KT keys x 32 queries] = K Q^T          O^T [dh x 32 queries] += V^T P^T
 // In the accumulator layout a lane holds 16 keys of ONE query, and they are the keys that the second product wants from this lane as
@@ -18,7 +18,7 @@
 // wave per SIMD) 532 us; products of one tile between the exponentials of the one before 562 us; fragments requested where they are used
 // 502 us, 4 keys' and 2 values' products ahead 495 us; of 499 us, 29 were the softmax's arithmetic and 126 waiting for LDS.
 // 256 prompts of 1 .. 512 tokens, 8 heads of 64: 78 us, 3.4 TB/s, half of it waiting: a workgroup has few tiles, and nearly all of them pass
-// the diagonal.  In fp32, 16 prompts of 1 .. 60 tokens, 2 heads of 128: 12.7 us (a tile of 32 keys 3.7 us, a third of it its products); 8
+// the diagonal.  In fp32, 16 prompts of 1 .. 60 tokens, 2 heads of 128: 12.6 us (a tile of 32 keys 3.7 us, a third of it its products); 8
 // prompts of 2048, 8 heads of 64: 134 TFLOP/s.
 //
 // fp32 inputs are split into three bf16 pieces (8 + 8 + 8 bits of significand, exactly the fp32 value) when a tile is staged, and the six
@@ -536,6 +536,13 @@ int launch_prompt(const PromptArgs& a, hipStream_t st, const char* who) {
         if (a.dh < 128) return launch_one<T, 128, 64, false>(a, st, who);
         return launch_one<T, 256, 32, false>(a, st, who);
     } else {
+        // The same, but here a tile costs its wave the splitting into pieces too: only where there are more workgroups than the GPU holds at once
+        // (256 prompts of 32 tokens, 16 heads over 4 of 128: 78 us, 139 with four waves; 8 heads of 64: 23 and 30; 16 prompts: 6.6 and 6.0).
+        if (a.N / a.B <= 32 && (int64_t)a.B * a.heads >= 1024) {
+            if (a.dh <= 32) return launch_one<T, 32, 32, false, 1>(a, st, who);
+            if (a.dh <= 64) return launch_one<T, 64, 32, false, 1>(a, st, who);
+            if (a.dh <= 128) return launch_one<T, 128, 32, false, 1>(a, st, who);
+        }
         if (a.dh <= 32) return launch_one<T, 32, 64, false>(a, st, who);
         if (a.dh <= 64) return launch_one<T, 64, 32, false>(a, st, who);
         if (a.dh <= 128) return launch_one<T, 128, 32, false>(a, st, who);
