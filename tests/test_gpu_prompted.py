@@ -315,6 +315,19 @@ def test_page_plan_short_lists_negative_lengths_no_room(K):
     assert small[2].tolist() == want[2][:20] and small[1].tolist() == want[1]
 
 
+@pytest.mark.parametrize('B', [3, 1030])
+def test_page_plan_room_beyond_31_bits(K, B):
+    """A length and a room whose sum passes 2^31: as many pages as the table is wide."""
+    top = 2 ** 31 - 1
+    lens, room, width, page = [5, 40, 0] + [1] * (B - 3), [top, top, top] + [0] * (B - 3), 4, 32
+    pages = list(range(100, 100 + 3 * width + B))
+    table, cu, slots, pos, seq, used = (torch.empty(s, dtype=torch.int32, device='cuda') for s in ((B, width), B + 1, sum(lens), sum(lens), sum(lens), 1))
+    K.page_plan(i32(lens), i32(room), i32(pages), page, table, cu, slots, pos, seq, used)
+    want = [pages[width * b:width * b + width] for b in range(3)] + [[pages[3 * width + b], -1, -1, -1] for b in range(B - 3)]
+    assert table.tolist() == want and used.item() == 3 * width + B - 3
+    assert slots.tolist()[:45] == [pages[0] * page + i for i in range(5)] + [pages[width + i // page] * page + i % page for i in range(40)]
+
+
 def test_page_step(K):
     table = i32([[5, 9, -1], [7, -1, -1], [2, 3, 4]])
     base, sent = i32([14, 16, 0]), i32([2, 0, 1, 9, -1, 0])

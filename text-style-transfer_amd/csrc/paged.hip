@@ -4,8 +4,8 @@
 // workgroup first adds up the tokens and pages of ALL sequences in front of its group: at most a few thousand lengths out of
 // the L2, cheaper than a second launch that would wait for a scan.  Then it scans its own group in LDS and writes table rows
 // and token entries; a lane takes four adjacent tokens, one search and three 16-byte stores.
-// 8192 sequences, 2.1 M tokens (27 MB): 12.2 us, 18.8 with one token per lane; 48 sequences: 5.2 us, a launch and the chain of loads
-// lengths -> offsets -> pages.
+// 8192 sequences, 2.1 M tokens (27 MB): 10.8 us, of which the sums in front of the groups are 4; 18.8 with one token per lane.  48
+// sequences: 4.5 us, a launch and the chain of loads lengths -> offsets -> pages.
 #include "tst_common.h"
 
 namespace {
@@ -20,14 +20,17 @@ struct PlanArgs {
     int aligned_in, aligned_out;    // lens and room / slots, pos and seq start at 16-byte boundaries
 };
 
-__device__ __forceinline__ int64_t need_of(const PlanArgs& a, int len, int room) {
-    const int64_t need = ((int64_t)max(len, 0) + max(room, 0) + (1 << a.page_shift) - 1) >> a.page_shift;
-    return need < a.width ? need : a.width;
+// pages of a sequence, in 32 bits: len + room may pass 2^31
+__device__ __forceinline__ int32_t need_of(const PlanArgs& a, int len, int room) {
+    const uint32_t n = (uint32_t)max(len, 0), r = (uint32_t)max(room, 0), m = (1u << a.page_shift) - 1u;
+    const uint32_t need = (n >> a.page_shift) + (r >> a.page_shift) + (((n & m) + (r & m) + m) >> a.page_shift);
+    return (int32_t)min(need, (uint32_t)a.width);
 }
 __device__ __forceinline__ int32_t clip31(int64_t v) { return v > 0x7fffffff ? 0x7fffffff : (int32_t)v; }
 
-__global__ __launch_bounds__(256) void page_plan_kernel(PlanArgs a) {
-    __shared__ int64_t part[2][4];
+template <int NT>
+__global__ __launch_bounds__(NT) void page_plan_kernel(PlanArgs a) {
+    __shared__ int64_t part[2][NT / 64];
     __shared__ int tok0[MAX_GROUP + 1], page0[MAX_GROUP + 1];      // within the group; entries behind its last sequence hold the totals
     const int t = threadIdx.x, lane = t & 63;
     const int64_t b0 = (int64_t)blockIdx.x * a.group;
@@ -37,15 +40,15 @@ __global__ __launch_bounds__(256) void page_plan_kernel(PlanArgs a) {
     if (a.aligned_in) {
         const int64_t quads = b0 >> 2;
 #pragma unroll 4
-        for (int64_t i = t; i < quads; i += 256) {
+        for (int64_t i = t; i < quads; i += NT) {
             const int4 n = reinterpret_cast<const int4*>(a.lens)[i];
             const int4 m = a.room != nullptr ? reinterpret_cast<const int4*>(a.room)[i] : make_int4(0, 0, 0, 0);
             st += (int64_t)max(n.x, 0) + max(n.y, 0) + max(n.z, 0) + max(n.w, 0);
-            sp += need_of(a, n.x, m.x) + need_of(a, n.y, m.y) + need_of(a, n.z, m.z) + need_of(a, n.w, m.w);
+            sp += (int64_t)need_of(a, n.x, m.x) + need_of(a, n.y, m.y) + need_of(a, n.z, m.z) + need_of(a, n.w, m.w);
         }
         b = quads << 2;
     }
-    for (b += t; b < b0; b += 256) {
+    for (b += t; b < b0; b += NT) {
         const int n = a.lens[b];
         st += max(n, 0);
         sp += need_of(a, n, a.room != nullptr ? a.room[b] : 0);
@@ -72,7 +75,9 @@ __global__ __launch_bounds__(256) void page_plan_kernel(PlanArgs a) {
         if (lane == 63) { tok0[64] = clip31(in); page0[64] = clip31(ip); }
     }
     __syncthreads();
-    const int64_t t_base = part[0][0] + part[0][1] + part[0][2] + part[0][3], p_base = part[1][0] + part[1][1] + part[1][2] + part[1][3];
+    int64_t t_base = 0, p_base = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) { t_base += part[0][i]; p_base += part[1][i]; }
     if (blockIdx.y == 0) {
         if (t < nb) a.cu[b0 + t] = clip31(t_base + tok0[t]);
         if (t == 0 && b0 + nb == a.B) {
@@ -82,7 +87,7 @@ __global__ __launch_bounds__(256) void page_plan_kernel(PlanArgs a) {
     }
     // table rows of the group, entry by entry
     const int64_t cells = (int64_t)nb * a.width;
-    for (int64_t i = (int64_t)blockIdx.y * 256 + t; i < cells; i += (int64_t)gridDim.y * 256) {
+    for (int64_t i = (int64_t)blockIdx.y * NT + t; i < cells; i += (int64_t)gridDim.y * NT) {
         const int s = cells <= 0x7fffffff ? (int)((uint32_t)i / (uint32_t)a.width) : (int)(i / a.width);
         const int64_t j = i - (int64_t)s * a.width, at = p_base + page0[s] + j;
         a.table[(b0 + s) * a.width + j] = (page0[s] + j < page0[s + 1] && at < a.n_pages) ? a.pages[at] : -1;
@@ -90,7 +95,7 @@ __global__ __launch_bounds__(256) void page_plan_kernel(PlanArgs a) {
     // tokens of the group: lane quads of adjacent tokens, at multiples of four of the packed index
     const int mask = (1 << a.page_shift) - 1;
     const int64_t lo = t_base, hi = min(t_base + tok0[MAX_GROUP], a.N);
-    for (int64_t q = (lo >> 2) + (int64_t)blockIdx.y * 256 + t; 4 * q < hi; q += (int64_t)gridDim.y * 256) {
+    for (int64_t q = (lo >> 2) + (int64_t)blockIdx.y * NT + t; 4 * q < hi; q += (int64_t)gridDim.y * NT) {
         const int64_t i0 = max(4 * q, lo);
         const int r0 = (int)(i0 - lo);
         int s = 0;
@@ -181,11 +186,16 @@ extern "C" int tst_page_plan(const int32_t* lens, const int32_t* room, int64_t B
     int64_t group = 1;
     while (group < MAX_GROUP && group * 512 < B) group *= 2;
     const int64_t groups = B > 0 ? (B + group - 1) / group : 1;
-    int64_t slices = (N + B * width + groups * 4096 - 1) / (groups * 4096);   // about four quads of tokens per thread
+    // many sequences: larger workgroups, fewer of which read the lengths (8192 sequences: 1024 threads 10.8 us, 512 11.6, 256 12.2; 48: 4.9, 4.6
+    // and 4.5)
+    const int64_t nt = B > 1024 ? 1024 : 256, share = B > 1024 ? 8192 : 4096;            // threads; tokens and table cells of a workgroup
+    int64_t slices = (N + B * width + groups * share - 1) / (groups * share);
     slices = slices < 1 ? 1 : (slices > 1024 ? 1024 : slices);
     const PlanArgs a{lens, room, pages, table, cu, slots, pos, seq, used, B, n_pages, N, width, shift, (int)group,
                      tst_aligned16(lens) && tst_aligned16(room), tst_aligned16(slots) && tst_aligned16(pos) && tst_aligned16(seq)};
-    page_plan_kernel<<<dim3((unsigned)groups, (unsigned)slices), 256, 0, (hipStream_t)stream>>>(a);
+    const dim3 grid((unsigned)groups, (unsigned)slices);
+    if (nt == 1024) page_plan_kernel<1024><<<grid, 1024, 0, (hipStream_t)stream>>>(a);
+    else page_plan_kernel<256><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     return tst_after_launch("tst_page_plan");
 }
 
