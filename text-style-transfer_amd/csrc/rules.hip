@@ -4,6 +4,7 @@
 namespace {
 
 constexpr int CHUNK_L = 8192, NT_L = 512;   // columns and threads of a workgroup where there are many rows
+constexpr int LIST = 2048;                  // columns on the list
 constexpr uint32_t SEEN = 0x80000000u;   // counter bit: the token is in the prompt
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -53,7 +54,7 @@ __device__ __forceinline__ void store16(__bf16* p, const float (&x)[8]) {
 template <typename T, int CHUNK, int NT>
 __global__ __launch_bounds__(NT) void adjust_logits_kernel(const T* logits, int64_t ld, int V, tst_logit_rules a, T* out, int64_t ldo) {
     __shared__ __attribute__((aligned(16))) uint32_t count[CHUNK];
-    __shared__ uint16_t list[CHUNK];
+    __shared__ uint16_t list[LIST];
     __shared__ int listed;
     constexpr int E = 16 / (int)sizeof(T);
     const int t = threadIdx.x;
@@ -113,7 +114,10 @@ __global__ __launch_bounds__(NT) void adjust_logits_kernel(const T* logits, int6
         auto note = [&](int v, bool prompt) {
             if ((uint32_t)(v - lo) >= (uint32_t)n) return;
             const uint32_t old = prompt ? atomicOr(&count[v - v0], SEEN) : atomicAdd(&count[v - v0], 1u);
-            if (old == 0u) list[atomicAdd(&listed, 1)] = (uint16_t)(v - v0);
+            if (old == 0u) {
+                const int at = atomicAdd(&listed, 1);
+                if (at < LIST) list[at] = (uint16_t)(v - v0);
+            }
         };
 #pragma unroll
         for (int u = 0; u < 4; ++u) note(vp[u], true);
@@ -132,9 +136,11 @@ __global__ __launch_bounds__(NT) void adjust_logits_kernel(const T* logits, int6
             for (int u = 0; u < 4; ++u) note(vh[u], false);
         }
         __syncthreads();
-        for (int i = t; i < listed; i += NT) {
-            const int at = list[i];
+        const bool all = listed > LIST;                              // more than the list holds: look at every column
+        for (int i = t; i < (all ? CHUNK : listed); i += NT) {
+            const int at = all ? i : list[i];
             const uint32_t c = count[at];
+            if (c == 0u) continue;
             float y = load1(row_in + v0 + at);
             y = y > 0.0f ? y / rp : y * rp;
             if ((c & ~SEEN) != 0u) y = (y - (float)(c & ~SEEN) * fp) - pp;
