@@ -684,6 +684,25 @@ def test_logit_rules_many_rows(K):
     assert torch.equal(out, y)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('R,n_hist', [(513, 9000), (300, 2500), (40, 9000), (520, 2049)])
+def test_logit_rules_long_histories(K, R, n_hist, dtype):
+    """Histories with more different tokens than a chunk's list holds, and just about as many."""
+    V = 9001
+    x = torch.randn((R, V), generator=gen(1), device='cuda').to(dtype)
+    hist = torch.randint(0, V, (R, n_hist), generator=gen(2), device='cuda', dtype=torch.int32)
+    hist[0] = torch.arange(n_hist, device='cuda', dtype=torch.int32) % V
+    hist[1] = 5
+    params = torch.rand((R, 3), generator=gen(3), device='cuda') + 1
+    out = torch.empty_like(x)
+    K.adjust_logits(x, R, V, out, params=params, hist=hist)
+    c = torch.zeros((R, V), device='cuda').scatter_add_(1, hist.long(), torch.ones((R, n_hist), device='cuda'))
+    f = x.float()
+    y = torch.where(c > 0, torch.where(f > 0, f / params[:, :1], f * params[:, :1]), f)
+    y = torch.where(c > 0, (y - c * params[:, 1:2]) - params[:, 2:3], y).to(dtype)
+    assert torch.equal(out, y)
+
+
 def test_grammar_next(K):
     table = i32([[1, -1, 2], [0, 2, 2], [-1, -1, -1]])
     state = i32([0, 1, 2, -1])

@@ -4,7 +4,7 @@
 namespace {
 
 constexpr int CHUNK_L = 8192, NT_L = 512;   // columns and threads of a workgroup where there are many rows
-constexpr int LIST = 2048;                  // columns on the list
+constexpr int LIST = 2048;                  // columns that the list holds
 constexpr uint32_t SEEN = 0x80000000u;   // counter bit: the token is in the prompt
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -48,9 +48,10 @@ __device__ __forceinline__ void store16(__bf16* p, const float (&x)[8]) {
 // Chunks begin where the row's addresses are 16-byte aligned, whatever the row's own alignment (`shift` columns before it); a row is only
 // handled element by element where logits and out are aligned differently.  In place (`out` is `logits`), pieces that no rule changes
 // are neither read nor written.
-// 2048 rows of 32000 bf16 logits with bias, masks and 1300 tokens each: 72 us, 3.6 TB/s; without rules 50 (a copy: 50), the bias 6, the tokens
-// 12 to 17 of it.  Measured beside it: the bias requested with the logits 80 us, chunks of 4096 with 256 threads 78, each workgroup taking
-// rows in turn with the next one's inputs under way 128, the simple kernel, a branch per column, 322.
+// 2048 rows of 32000 bf16 logits with bias, masks and 1300 tokens each: 69.7 us, 3.8 TB/s; without rules 50 (a copy: 50), the bias 7, the
+// tokens 9 to 13 of it.  The list is short so that four workgroups share a CU (with room for every column, three: 72.5).  Measured beside
+// it: the bias requested with the logits 80 us, after the counting 74, chunks of 4096 with 256 threads 78, each workgroup taking rows in
+// turn with the next one's inputs under way 128, the simple kernel, a branch per column, 322.
 template <typename T, int CHUNK, int NT>
 __global__ __launch_bounds__(NT) void adjust_logits_kernel(const T* logits, int64_t ld, int V, tst_logit_rules a, T* out, int64_t ldo) {
     __shared__ __attribute__((aligned(16))) uint32_t count[CHUNK];
