@@ -660,7 +660,8 @@ __global__ __launch_bounds__(512) void attn_cache4_combine_kernel(AttendArgs a) 
 
 // How a call is cut: tokens per workgroup (chunk) and how many chunks the longest row may have.  Few (row, key head) units: as many
 // workgroups as run at once, two to a CU, since every chunk costs a prologue and a partial result (3 rows x 4 key heads, 131001
-// tokens: 36.8 us at 512 workgroups; before the partial results were requested early 38.8, 41.5 at 1024, 46.7 at 1536).  Many: 1024, so that rows of different lengths even out, and whole
+// tokens: 36.8 us at 512 workgroups; before the partial results were requested early 38.8, 41.5 at 1024, 46.7 at 1536).  Many: 1024, so
+// that rows of different lengths even out, and whole
 // rows up to 8192 tokens once there are that many units (256 rows x 8 key heads, up to 8000 tokens: 219 us in one piece, 225 cut at
 // 4096, 231 at 2048).  At least one tile for each of the four waves.
 void cut(int64_t R, int64_t kv_heads, int64_t head_groups, int64_t max_len, int* chunk, int* splits) {

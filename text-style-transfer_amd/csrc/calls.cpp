@@ -176,7 +176,8 @@ void attn_prompt(PyObject* const* a) {
     disjoint(ro.p, ro.ld, rv.p, rv.ld, N, wq, wk, size, "out must not overlap q, k or v");
     const float scale = scale_or(a[7], dh);
     void* st = current_stream(dev);
-    if (low) issue("tst_attn_prompt_bf16", entry.tst_attn_prompt_bf16, rq.p, rq.ld, rk.p, rk.ld, rv.p, rv.ld, cu, n_cu - 1, ro.p, ro.ld, N, heads, kv_heads, dh, scale, st);
+    if (low) issue("tst_attn_prompt_bf16", entry.tst_attn_prompt_bf16, rq.p, rq.ld, rk.p, rk.ld, rv.p, rv.ld, cu, n_cu - 1, ro.p, ro.ld, N, heads, kv_heads,
+                   dh, scale, st);
     else issue("tst_attn_prompt_f32", entry.tst_attn_prompt_f32, (const float*)rq.p, rq.ld, (const float*)rk.p, rk.ld, (const float*)rv.p, rv.ld, cu, n_cu - 1,
                (float*)ro.p, ro.ld, N, heads, kv_heads, dh, scale, st);
 }
@@ -259,7 +260,8 @@ void attn_cache4(PyObject* const* a) {
     const int32_t *seq = ints(a[9], n, dev, "seq"), *lens = ints(a[4], n, dev, "lens");
     const float scale = scale_or(a[10], dh);
     void* st = current_stream(dev);
-    if (low) issue("tst_attn_cache4_bf16", entry.tst_attn_cache4_bf16, c, rq.p, rq.ld, t.p, t.width, t.rows, seq, lens, max_len, ro.p, ro.ld, n, heads, scale, work, n_work, st);
+    if (low) issue("tst_attn_cache4_bf16", entry.tst_attn_cache4_bf16, c, rq.p, rq.ld, t.p, t.width, t.rows, seq, lens, max_len, ro.p, ro.ld, n, heads, scale,
+                   work, n_work, st);
     else issue("tst_attn_cache4_f32", entry.tst_attn_cache4_f32, c, (const float*)rq.p, rq.ld, t.p, t.width, t.rows, seq, lens, max_len, (float*)ro.p, ro.ld, n, heads,
                scale, work, n_work, st);
 }

@@ -14,9 +14,10 @@
 //
 // What bounds it (dh 128, bf16): 64 keys x 32 queries cost a SIMD 1024 cycles of matrix instructions, and the four SIMDs together 1024
 // cycles of LDS reads (128 bytes per cycle), so both run full at the limit.  Two prompts of up to 8191 tokens, 16 heads over 4 key heads:
-// 479 .. 496 us, 1.10 .. 1.14 PFLOP/s, the rate of a large library product here (29.8 ms plainly).  Measured on the way: a running maximum 595 us; 64 queries per wave (half the LDS reads, but one
-// wave per SIMD) 532 us; products of one tile between the exponentials of the one before 562 us; fragments requested where they are used
-// 502 us, 4 keys' and 2 values' products ahead 495 us; of 499 us, 29 were the softmax's arithmetic and 126 waiting for LDS.
+// 479 .. 496 us, 1.10 .. 1.14 PFLOP/s, the rate of a large library product here (29.8 ms plainly).  Measured on the way: a running
+// maximum 595 us; 64 queries per wave (half the LDS reads, but one wave per SIMD) 532 us; products of one tile between the exponentials
+// of the one before 562 us; workgroups of two waves 583 us; fragments requested where they are used 502 us, 4 keys' and 2 values'
+// products ahead 495 us; of 499 us, 29 were the softmax's arithmetic and 126 waiting for LDS.
 // 256 prompts of 1 .. 512 tokens, 8 heads of 64: 78 us, 3.4 TB/s, half of it waiting: a workgroup has few tiles, and nearly all of them pass
 // the diagonal.  In fp32, 16 prompts of 1 .. 60 tokens, 2 heads of 128: 12.6 us (a tile of 32 keys 3.7 us, a third of it its products); 8
 // prompts of 2048, 8 heads of 64: 134 TFLOP/s.
