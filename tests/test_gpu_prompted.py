@@ -208,7 +208,7 @@ def test_prompt_short_alone_and_beside_a_long_one(K, heads, kv_heads, dh, dtype)
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize('heads,kv_heads,dh', [(8, 4, 32), (8, 8, 24), (8, 2, 64), (16, 4, 128), (8, 1, 72)])
+@pytest.mark.parametrize('heads,kv_heads,dh', [(8, 4, 32), (8, 8, 24), (8, 2, 64), (16, 4, 128), (8, 1, 72), (8, 1, 256), (12, 2, 128)])
 def test_prompt_many_short(K, heads, kv_heads, dh, dtype):
     """Enough short prompts to fill the GPU several times; some longer than a tile, some empty."""
     lens = ([3, 17, 0, 32, 33, 1, 66, 8] * 17)[:130]

@@ -151,9 +151,10 @@ __device__ __forceinline__ void one_row(const PromptArgs& a, int64_t c0, int64_t
 }
 
 // DMA: bf16 rows of exactly DH elements go from memory to LDS without registers, two buffers; else through registers, one buffer.
-template <typename T, int DH, int KT, bool DMA, int WAVES>
+// PACKED: the waves of a workgroup take the same 32 rows of adjacent heads that share a key head.
+template <typename T, int DH, int KT, bool DMA, int WAVES, bool PACKED>
 __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_prompt_kernel(PromptArgs a) {
-    constexpr int NT = 64 * WAVES, BM = 32 * WAVES;  // threads, rows per workgroup
+    constexpr int NT = 64 * WAVES, BM = PACKED ? 32 : 32 * WAVES;      // threads, rows per workgroup
     constexpr int NP = sizeof(T) == 4 ? 3 : 1;
     constexpr int CH = DH / 8;                       // chunks per row of a tile
     constexpr int PLANE = KT * DH * 2;               // bytes of one piece of a tile
@@ -173,21 +174,24 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
     // so reads whole rows.  (Prompts of 1 .. 512 tokens, 8 heads of 64: 78 us by rows, 82.5 by heads; of 8191, 16 heads of 128: 513 and 484.)
     // The last, longest row tiles of a sequence come first.
     uint32_t id = blockIdx.x;
-    int head;
+    int head;                                        // PACKED: the first of WAVES adjacent ones
+    const uint32_t heads = (uint32_t)a.heads / (PACKED ? WAVES : 1), per_kv = (uint32_t)a.per_kv / (PACKED ? WAVES : 1);
     if (a.by_rows) {
         const uint32_t xcd = id & 7u;
         id >>= 3;
-        head = (int)(id % (uint32_t)a.heads);
-        id /= (uint32_t)a.heads;
+        head = (int)(id % heads);
+        id /= heads;
         id = id * 8u + ((xcd + 3u * id) & 7u);   // rotated, so that tiles without rows, every second or third for some lengths, meet every XCD
         if (id >= (uint32_t)a.tiles) return;
     } else {
         const int key_head = (int)(id % (uint32_t)a.kv_heads);
         id /= (uint32_t)a.kv_heads;
-        head = key_head * a.per_kv + (int)(id % (uint32_t)a.per_kv);
-        id /= (uint32_t)a.per_kv;
+        head = key_head * (int)per_kv + (int)(id % per_kv);
+        id /= per_kv;
     }
+    if (PACKED) head *= WAVES;
     const int g = head / a.per_kv;
+    if (PACKED) head += w;
     id = (uint32_t)a.tiles - 1u - id;
     // Sequence b owns tile numbers from cu[b] / BM + b on: strictly ascending, and always enough of them.  A search by 64 probes at once, the
     // last of which also hold the sequence's ends: one load for up to 64 sequences, two for 4096.
@@ -209,7 +213,7 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
     const int64_t qt = (int64_t)id - (c0 / BM + lo);
     if (c0 < 0 || c1 > a.N || qt < 0 || qt * BM >= c1 - c0) return;      // the whole workgroup
     const int len = (int)(c1 - c0);
-    const int q0 = (int)qt * BM, qw = q0 + 32 * w, row = qw + col;                     // first row of the workgroup and of this wave, this lane's row (in the sequence)
+    const int q0 = (int)qt * BM, qw = q0 + (PACKED ? 0 : 32 * w), row = qw + col;      // workgroup's, wave's first, lane's row
     const int q_end = min(q0 + BM, len) - 1, w_end = min(qw + 32, len) - 1;
 
     const T* kp = (const T*)a.k + c0 * a.ldk + (int64_t)g * a.dh;
@@ -506,29 +510,37 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
         one_row<T>(a, c0, c0 + qw + __builtin_ctz(cols), head, g);
 }
 
-template <typename T, int DH, int KT, bool DMA, int WAVES = 4>
+template <typename T, int DH, int KT, bool DMA, int WAVES = 4, bool PACKED = false>
 int launch_one(PromptArgs a, hipStream_t st, const char* who) {
-    constexpr int BM = 32 * WAVES;
+    constexpr int BM = PACKED ? 32 : 32 * WAVES;
     const int64_t tiles = a.N / BM + a.B;                                   // sequence b owns tiles cu[b] / BM + b ..
     a.by_rows = a.N / a.B * a.kv_heads * a.dh * 2 * (int64_t)sizeof(T) <= (1 << 21);
-    const int64_t groups = (a.by_rows ? (tiles + 7) / 8 * 8 : tiles) * a.heads;
+    const int64_t groups = (a.by_rows ? (tiles + 7) / 8 * 8 : tiles) * (a.heads / (PACKED ? WAVES : 1));
     TST_REQUIRE(groups <= (int64_t)0x7fffffff, TST_ERR_UNSUPPORTED, "%s: too many row tiles", who);
     a.tiles = (int)tiles;
-    attn_prompt_kernel<T, DH, KT, DMA, WAVES><<<(unsigned)groups, 64 * WAVES, 0, st>>>(a);
+    attn_prompt_kernel<T, DH, KT, DMA, WAVES, PACKED><<<(unsigned)groups, 64 * WAVES, 0, st>>>(a);
     return tst_after_launch(who);
 }
 
 template <typename T>
 int launch_prompt(const PromptArgs& a, hipStream_t st, const char* who) {
+    // More workgroups of four waves of rows than the GPU holds at once (those of 128 elements and more in fp32, of 256 in bf16: one per CU)
+    const bool many = (a.N / 128 + a.B) * a.heads > (a.dh > (sizeof(T) == 4 ? 64 : 128) ? 256 : 512);
+    // Such calls with few rows per prompt, where most waves would have none: the waves take four heads that share a key head instead, which
+    // also stages the keys (in fp32: splits them) once for the four.  Prompts of 16 tokens, one wave or four / packed: fp32, 16 heads over 4
+    // of 128, 16 prompts 16.8 / 10.5 us, 256 prompts 75 / 45; 8 over 2 of 64, 72 prompts 10.5 / 6.9; bf16, 4 over 1 of 256, 72 prompts 11.7 / 8.1.
+    // Of 96 tokens: 33 / 21, 283 / 207, 23.5 / 22, 20.9 / 25; calls that fit at once lose (fp32, 8 over 2 of 64, 16 prompts of 16: 5.6 / 6.6).
+    const bool packed = many && a.per_kv % 4 == 0 && a.N / a.B <= (sizeof(T) == 4 ? 96 : 64);
     if constexpr (sizeof(T) == 2) {
         // Prompts of a few rows: one wave per workgroup, one tile of 32 keys in LDS, so that many are at work (256 prompts, 32 heads over 8 of
-        // 128: 2 tokens each 19 us, 62 with four waves; 32 tokens 33 and 76; 48 tokens 57 and 90; 96 tokens 142 and 158, but of 8 heads of 64
+        // 128: 2 tokens each 19 us, 62 with four waves; 32 tokens 33 and 76; 64 tokens 91 and 120; 96 tokens 142 and 158, but of 8 heads of 64
         // 27 and 23).  A row's sums run over the same keys in the same order either way.
-        if (a.N / a.B <= 48) {
+        if (a.N / a.B <= 64) {
             if (a.dh == 32) return launch_one<T, 32, 32, true, 1>(a, st, who);
             if (a.dh == 64) return launch_one<T, 64, 32, true, 1>(a, st, who);
             if (a.dh == 128) return launch_one<T, 128, 32, true, 1>(a, st, who);
         }
+        if (packed && a.dh == 256) return launch_one<T, 256, 32, true, 4, true>(a, st, who);
         if (a.dh == 32) return launch_one<T, 32, 64, true>(a, st, who);
         if (a.dh == 64) return launch_one<T, 64, 64, true>(a, st, who);
         if (a.dh == 128) return launch_one<T, 128, 64, true>(a, st, who);
@@ -537,9 +549,14 @@ int launch_prompt(const PromptArgs& a, hipStream_t st, const char* who) {
         if (a.dh < 128) return launch_one<T, 128, 64, false>(a, st, who);
         return launch_one<T, 256, 32, false>(a, st, who);
     } else {
-        // The same, but here a tile costs its wave the splitting into pieces too: only where there are more workgroups than the GPU holds at once
-        // (256 prompts of 32 tokens, 16 heads over 4 of 128: 78 us, 139 with four waves; 8 heads of 64: 23 and 30; 16 prompts: 6.6 and 6.0).
-        if (a.N / a.B <= 32 && (int64_t)a.B * a.heads >= 1024) {
+        if (packed && a.dh > 32) {                       // (not for heads of 256 elements: registers)
+            if (a.dh <= 64) return launch_one<T, 64, 32, false, 4, true>(a, st, who);
+            if (a.dh <= 128) return launch_one<T, 128, 32, false, 4, true>(a, st, who);
+        }
+        // One wave per workgroup as in bf16, but here a tile costs its wave the splitting into pieces too: only where there are more workgroups
+        // than the GPU holds at once (256 prompts of 32 tokens, 16 heads of 128: 78 us, 139 with four waves; 8 of 64: 23 and 30; 16 prompts: 6.6
+        // and 6.0).
+        if (many && a.N / a.B <= 32) {
             if (a.dh <= 32) return launch_one<T, 32, 32, false, 1>(a, st, who);
             if (a.dh <= 64) return launch_one<T, 64, 32, false, 1>(a, st, who);
             if (a.dh <= 128) return launch_one<T, 128, 32, false, 1>(a, st, who);
