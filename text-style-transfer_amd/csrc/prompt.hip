@@ -19,8 +19,8 @@
 // of the one before 562 us; workgroups of two waves 583 us; fragments requested where they are used 502 us, 4 keys' and 2 values'
 // products ahead 495 us; of 499 us, 29 were the softmax's arithmetic and 126 waiting for LDS.
 // 256 prompts of 1 .. 512 tokens, 8 heads of 64: 78 us, 3.4 TB/s, half of it waiting: a workgroup has few tiles, and nearly all of them pass
-// the diagonal.  In fp32, 16 prompts of 1 .. 60 tokens, 2 heads of 128: 12.6 us (a tile of 32 keys 3.7 us, a third of it its products); 8
-// prompts of 2048, 8 heads of 64: 134 TFLOP/s.
+// the diagonal.  In fp32, 16 prompts of 1 .. 60 tokens, 2 heads of 128: 10.0 us; 8 prompts of 2048, 8
+// heads of 64: 139 TFLOP/s, of 128: 124.  (With loads under a condition for heads smaller than the tile 12.6 us, 134 and 107.)
 //
 // fp32 inputs are split into three bf16 pieces (8 + 8 + 8 bits of significand, exactly the fp32 value) when a tile is staged, and the six
 // products of pieces down to 2^-18 of the largest are summed in fp32: what is left out is below 2^-26 of each product, and six bf16
@@ -250,13 +250,15 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
     float4 stage_k2[NP == 3 ? PER : 1], stage_v2[NP == 3 ? PER : 1];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
     const int wu = __builtin_amdgcn_readfirstlane(w);
-    // a lane's byte offsets within a whole tile never change: the tile's own address is scalar
+    // A lane's byte offsets within a whole tile never change: the tile's own address is scalar.  Chunks behind the head read its last elements
+    // again: the query is 0 there, and such outputs are not stored.
     uint32_t off_k[PER], off_v[PER];
+    constexpr int PIECE = 16 / (int)sizeof(T);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int x = threadIdx.x + NT * j, r = x / CH, c = x % CH;
-        off_k[j] = (uint32_t)(r * (int)a.ldk + 8 * (DMA ? c ^ k_swizzle<DH>(r) : c)) * (uint32_t)sizeof(T);
-        off_v[j] = (uint32_t)(r * (int)a.ldv + 8 * (DMA ? c ^ v_swizzle<DH>(r) : c)) * (uint32_t)sizeof(T);
+        off_k[j] = (uint32_t)(r * (int)a.ldk + (DMA ? 8 * (c ^ k_swizzle<DH>(r)) : min(8 * c, a.dh - PIECE))) * (uint32_t)sizeof(T);
+        off_v[j] = (uint32_t)(r * (int)a.ldv + (DMA ? 8 * (c ^ v_swizzle<DH>(r)) : min(8 * c, a.dh - PIECE))) * (uint32_t)sizeof(T);
     }
     auto fetch = [&](int k0, int buf) {
         const unsigned char* tk = reinterpret_cast<const unsigned char*>(kp + (int64_t)k0 * a.ldk);
@@ -278,13 +280,12 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
             } else {
                 const unsigned char* sk = tk + (int64_t)(int32_t)ok;
                 const unsigned char* sv = tv + (int64_t)(int32_t)ov;
-                const u32x4 zero = {0u, 0u, 0u, 0u};
-                stage_k[j] = 8 * c < a.dh ? *reinterpret_cast<const u32x4*>(sk) : zero;
-                stage_v[j] = 8 * c < a.dh ? *reinterpret_cast<const u32x4*>(sv) : zero;
+                stage_k[j] = *reinterpret_cast<const u32x4*>(sk);
+                stage_v[j] = *reinterpret_cast<const u32x4*>(sv);
                 if (NP == 3) {
-                    const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                    stage_k2[j] = 8 * c + 4 < a.dh ? *reinterpret_cast<const float4*>(sk + 16) : z;
-                    stage_v2[j] = 8 * c + 4 < a.dh ? *reinterpret_cast<const float4*>(sv + 16) : z;
+                    const int second = 8 * c + 4 < a.dh ? 16 : 0;
+                    stage_k2[j] = *reinterpret_cast<const float4*>(sk + second);
+                    stage_v2[j] = *reinterpret_cast<const float4*>(sv + second);
                 }
             }
         }
