@@ -20,7 +20,7 @@
 // products ahead 495 us; of 499 us, 29 were the softmax's arithmetic and 126 waiting for LDS.
 // 256 prompts of 1 .. 512 tokens, 8 heads of 64: 78 us, 3.4 TB/s, half of it waiting: a workgroup has few tiles, and nearly all of them pass
 // the diagonal.  In fp32, 16 prompts of 1 .. 60 tokens, 2 heads of 128: 10.0 us; 8 prompts of 2048, 8
-// heads of 64: 139 TFLOP/s, of 128: 124.  (With loads under a condition for heads smaller than the tile 12.6 us, 134 and 107.)
+// heads of 64: 142 TFLOP/s, of 128: 129.  (With loads under a condition for heads smaller than the tile 12.6 us, 134 and 107.)
 //
 // fp32 inputs are split into three bf16 pieces (8 + 8 + 8 bits of significand, exactly the fp32 value) when a tile is staged, and the six
 // products of pieces down to 2^-18 of the largest are summed in fp32: what is left out is below 2^-26 of each product, and six bf16
@@ -55,10 +55,10 @@ __device__ __forceinline__ float high_f(uint32_t u) { return __uint_as_float(u &
 
 // Eight elements as NP pieces of eight bf16.  What is not finite, or rounds to infinity, leaves a NaN in the second piece, which every product
 // passes on: rows that meet it are computed again, plainly.
-__device__ __forceinline__ void split8(const float (&x)[8], bool negate, Frag (&f)[3]) {
+__device__ __forceinline__ void split8(const float (&x)[8], Frag (&f)[3]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        float a = negate ? -x[2 * e] : x[2 * e], b = negate ? -x[2 * e + 1] : x[2 * e + 1];
+        float a = x[2 * e], b = x[2 * e + 1];
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
             f[i].u[e] = pack2(a, b);
@@ -67,20 +67,14 @@ __device__ __forceinline__ void split8(const float (&x)[8], bool negate, Frag (&
         }
     }
 }
-__device__ __forceinline__ void pieces(const float* p, int have, bool negate, Frag (&f)[3]) {
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-        const float4 v = e < have ? *reinterpret_cast<const float4*>(p + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[e] = v.x; x[e + 1] = v.y; x[e + 2] = v.z; x[e + 3] = v.w;
-    }
-    split8(x, negate, f);
-}
-__device__ __forceinline__ void pieces(const __bf16* p, int have, bool negate, Frag (&f)[1]) {
-    f[0].q = have >= 8 ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t signs = negate ? 0x80008000u : 0u;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[0].u[e] ^= signs;
+// 16 bytes of a head of dh elements at element `at`, zeros behind it, with flipped signs or not.  The load is never under a condition: such
+// loads wait for each other.
+template <typename T>
+__device__ __forceinline__ uint4 query16(const T* head, int at, int dh, uint32_t signs) {
+    uint4 v = *reinterpret_cast<const uint4*>(head + min(at, dh - 16 / (int)sizeof(T)));
+    const uint32_t keep = at < dh ? 0xffffffffu : 0u;
+    v.x = (v.x ^ signs) & keep; v.y = (v.y ^ signs) & keep; v.z = (v.z ^ signs) & keep; v.w = (v.w ^ signs) & keep;
+    return v;
 }
 
 struct PromptArgs {
@@ -225,14 +219,20 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
     Frag q[KS][WHOLE ? 2 : NP];
     {
         const T* qp = (const T*)a.q + (c0 + min(row, len - 1)) * a.ldq + (int64_t)head * a.dh;
+        const uint32_t signs = a.negate == 0 ? 0u : (NP == 3 ? 0x80000000u : 0x80008000u);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            if constexpr (WHOLE) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    q[s][e].q = 16 * s + 8 * h + 4 * e < a.dh ? *reinterpret_cast<const uint4*>(qp + 16 * s + 8 * h + 4 * e) : make_uint4(0u, 0u, 0u, 0u);
+            const int at = 16 * s + 8 * h;
+            if constexpr (NP == 1) {
+                q[s][0].q = query16(qp, at, a.dh, signs);
+            } else if constexpr (WHOLE) {
+                q[s][0].q = query16(qp, at, a.dh, signs);
+                q[s][1].q = query16(qp, at + 4, a.dh, signs);
             } else {
-                pieces(qp + 16 * s + 8 * h, a.dh - (16 * s + 8 * h), a.negate != 0, q[s]);
+                const uint4 u = query16(qp, at, a.dh, signs), v = query16(qp, at + 4, a.dh, signs);
+                const float e8[8] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w),
+                                     __uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+                split8(e8, q[s]);
             }
         }
     }
@@ -385,7 +385,7 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
                             asm volatile("" : "+v"(u));              // or the compiler would split them all before the loop
                             e8[e] = __uint_as_float(u);
                         }
-                        split8(e8, a.negate != 0, split);
+                        split8(e8, split);
                     }
                     const auto& qs = [&]() -> const auto& { if constexpr (WHOLE) return split; else return q[s]; }();
 #pragma unroll
