@@ -528,14 +528,14 @@ int launch_prompt(const PromptArgs& a, hipStream_t st, const char* who) {
     // More workgroups of four waves of rows than the GPU holds at once (those of 128 elements and more in fp32, of 256 in bf16: one per CU)
     const bool many = (a.N / 128 + a.B) * a.heads > (a.dh > (sizeof(T) == 4 ? 64 : 128) ? 256 : 512);
     // Such calls with few rows per prompt, where most waves would have none: the waves take four heads that share a key head instead, which
-    // also stages the keys (in fp32: splits them) once for the four.  Prompts of 16 tokens, one wave or four / packed: fp32, 16 heads over 4
-    // of 128, 16 prompts 16.8 / 10.5 us, 256 prompts 75 / 45; 8 over 2 of 64, 72 prompts 10.5 / 6.9; bf16, 4 over 1 of 256, 72 prompts 11.7 / 8.1.
-    // Of 96 tokens: 33 / 21, 283 / 207, 23.5 / 22, 20.9 / 25; calls that fit at once lose (fp32, 8 over 2 of 64, 16 prompts of 16: 5.6 / 6.6).
+    // also stages the keys (in fp32: splits them) once for the four.  Prompts of 16 tokens, four waves of rows / packed: fp32, 16 heads over 4 of
+    // 128, 16 prompts 13.1 / 8.3 us, 256 prompts 102 / 35; 8 over 2 of 64, 72 prompts 9.1 / 6.0; bf16, 4 over 1 of 256, 72 prompts 11.5 / 7.9.  Of 96
+    // tokens: 26.5 / 17.1, 214 / 158, 19.4 / 17.8, 20.1 / 24.9.  Calls that fit at once lose (fp32, 8 over 2 of 64, 16 of 16: 5.0 / 5.4).
     const bool packed = many && a.per_kv % 4 == 0 && a.N / a.B <= (sizeof(T) == 4 ? 96 : 64);
     if constexpr (sizeof(T) == 2) {
         // Prompts of a few rows: one wave per workgroup, one tile of 32 keys in LDS, so that many are at work (256 prompts, 32 heads over 8 of
-        // 128: 2 tokens each 19 us, 62 with four waves; 32 tokens 33 and 76; 64 tokens 91 and 120; 96 tokens 142 and 158, but of 8 heads of 64
-        // 27 and 23).  A row's sums run over the same keys in the same order either way.
+        // 128: 2 tokens each 19 us, 62 with four waves; 32 tokens 32 and 74; 64 tokens 86 and 110; 96 tokens 135 and 150, but of 8 heads of 64
+        // 27 and 22).  A row's sums run over the same keys in the same order either way.
         if (a.N / a.B <= 64) {
             if (a.dh == 32) return launch_one<T, 32, 32, true, 1>(a, st, who);
             if (a.dh == 64) return launch_one<T, 64, 32, true, 1>(a, st, who);
@@ -555,9 +555,9 @@ int launch_prompt(const PromptArgs& a, hipStream_t st, const char* who) {
             if (a.dh <= 128) return launch_one<T, 128, 32, false, 4, true>(a, st, who);
         }
         // One wave per workgroup as in bf16, but here a tile costs its wave the splitting into pieces too: only where there are more workgroups
-        // than the GPU holds at once (256 prompts of 32 tokens, 16 heads of 128: 78 us, 139 with four waves; 8 of 64: 23 and 30; 16 prompts: 6.6
-        // and 6.0).
-        if (many && a.N / a.B <= 32) {
+        // than the GPU holds at once (256 prompts of 32 tokens, 16 heads of 128: 60 us, 105 with four waves, of 64 tokens 142 and 162, of 96 238 and
+        // 229; 8 heads of 64: 18 and 25, 32 and 36, 51 and 48; 16 prompts of 32 tokens, 8 heads of 64: 5.6 and 5.1).
+        if (many && a.N / a.B <= 64) {
             if (a.dh <= 32) return launch_one<T, 32, 32, false, 1>(a, st, who);
             if (a.dh <= 64) return launch_one<T, 64, 32, false, 1>(a, st, who);
             if (a.dh <= 128) return launch_one<T, 128, 32, false, 1>(a, st, who);
