@@ -222,6 +222,18 @@ def test_prompt_many_short(K, heads, kv_heads, dh, dtype):
         assert torch.equal(part, out)
 
 
+@pytest.mark.parametrize('heads,kv_heads,dh,dtype', [(256, 64, 256, torch.bfloat16), (256, 64, 128, torch.float32), (128, 128, 128, torch.bfloat16),
+                                                     (80, 80, 128, torch.float32)])
+def test_prompt_short_with_wide_rows(K, heads, kv_heads, dh, dtype):
+    """Short prompts whose keys do not fit an L2 together: the other work order."""
+    lens, per = [40, 33, 70, 1, 50, 64], heads // kv_heads
+    q, k, v, cu, out = prompt_case(K, lens, heads, kv_heads, dh, dtype, seed=heads)
+    for h in (0, 1, per - 1, per, heads // 2 + 3, heads - per, heads - 1):
+        one, g = slice(h * dh, (h + 1) * dh), slice(h // per * dh, (h // per + 1) * dh)
+        check_prompt(q[:, one], k[:, g], v[:, g], cu, out[:, one], 1, 1, dh, dtype)
+    assert not (out == 7).all(1).any()
+
+
 @pytest.mark.parametrize('B', [63, 64, 65, 130, 4097])
 def test_prompt_many_sequences(K, B):
     g = torch.Generator().manual_seed(B)
