@@ -14,7 +14,7 @@
 //
 // What bounds it (dh 128, bf16): 64 keys x 32 queries cost a SIMD 1024 cycles of matrix instructions, and the four SIMDs together 1024
 // cycles of LDS reads (128 bytes per cycle), so both run full at the limit.  Two prompts of up to 8191 tokens, 16 heads over 4 key heads:
-// 479 .. 496 us, 1.10 .. 1.14 PFLOP/s, the rate of a large library product here (29.8 ms plainly).  Measured on the way: a running
+// 479 .. 513 us on different cards, 1.07 .. 1.14 PFLOP/s, the rate of a large library product (29.8 ms plainly).  Measured on the way: a running
 // maximum 595 us; 64 queries per wave (half the LDS reads, but one wave per SIMD) 532 us; products of one tile between the exponentials
 // of the one before 562 us; workgroups of two waves 583 us; fragments requested where they are used 502 us, 4 keys' and 2 values'
 // products ahead 495 us; of 499 us, 29 were the softmax's arithmetic and 126 waiting for LDS.
