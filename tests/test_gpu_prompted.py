@@ -222,6 +222,37 @@ def test_prompt_many_short(K, heads, kv_heads, dh, dtype):
         assert torch.equal(part, out)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('B', [3, 150])
+@pytest.mark.parametrize('heads,kv_heads,dh', [(8, 2, 64), (8, 8, 128), (8, 2, 128), (4, 1, 256), (8, 8, 32)])
+def test_prompt_short_nonfinite_and_steep(K, heads, kv_heads, dh, B, dtype):
+    """Short prompts, few and many: an infinity in the middle of one reaches only what attends to it; scores that rise by thousands of
+    powers of two, on values near the top of the range."""
+    L, w = 41, kv_heads * dh
+    g = gen(B)
+    q, k, v = (torch.randn((B * L, n), generator=g, device='cuda') for n in (heads * dh, w, w))
+    for h in range(heads):
+        q[L:2 * L, h * dh] = 1.0
+    for h in range(kv_heads):
+        k[L:2 * L, h * dh] = torch.arange(L, device='cuda') * 40.0
+    v[L:2 * L] *= 2.0 ** 100
+    k[20, 3], v[2 * L + 33, 1] = math.inf, math.nan
+    q[:L, 3] = q[:L, 3].abs() + 0.5
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    cu = list(range(0, B * L + 1, L))
+    out = torch.empty_like(q)
+    K.attn_prompt(q, k, v, i32(cu), out, heads, kv_heads, scale=1.0)
+    check_prompt(q[:20], k[:20], v[:20], [0, 20], out[:20], heads, kv_heads, dh, dtype, scale=1.0)
+    check_prompt(q, k, v, [L, 2 * L], out, heads, kv_heads, dh, dtype, scale=1.0)
+    check_prompt(q, k, v, [2 * L, 2 * L + 33], out, heads, kv_heads, dh, dtype, scale=1.0)
+    assert torch.isnan(out[20:L, :dh]).all() and torch.isnan(out[2 * L + 33:3 * L, 1]).all()
+    if kv_heads > 1:
+        last = (heads - 1) * dh
+        assert torch.isfinite(out[:L, last:]).all() and torch.isfinite(out[2 * L:3 * L, last:]).all()
+    if B > 3:
+        check_prompt(q, k, v, [(B - 1) * L, B * L], out, heads, kv_heads, dh, dtype, scale=1.0)
+
+
 @pytest.mark.parametrize('heads,kv_heads,dh,dtype', [(256, 64, 256, torch.bfloat16), (256, 64, 128, torch.float32), (128, 128, 128, torch.bfloat16),
                                                      (80, 80, 128, torch.float32)])
 def test_prompt_short_with_wide_rows(K, heads, kv_heads, dh, dtype):
