@@ -658,15 +658,17 @@ __global__ __launch_bounds__(512) void attn_cache4_combine_kernel(AttendArgs a) 
     }
 }
 
-// How a call is cut: tokens per workgroup (chunk) and how many chunks the longest row may have.  Few (row, key head) units: as many
-// workgroups as run at once, two to a CU, since every chunk costs a prologue and a partial result (3 rows x 4 key heads, 131001
-// tokens: 36.8 us at 512 workgroups; before the partial results were requested early 38.8, 41.5 at 1024, 46.7 at 1536).  Many: 1024, so
-// that rows of different lengths even out, and whole
-// rows up to 8192 tokens once there are that many units (256 rows x 8 key heads, up to 8000 tokens: 219 us in one piece, 225 cut at
-// 4096, 231 at 2048).  At least one tile for each of the four waves.
+// How a call is cut: tokens per workgroup (chunk) and how many chunks the longest row may have.  A second launch that joins chunks costs 3 us
+// and every chunk a prologue, so rows stay whole where walking one takes no longer: up to 1024 tokens (bf16, 4 key heads of 128, one row of
+// 512 tokens: 6.1 us whole, 8.6 cut; 1024 tokens: 8.0 and 8.7; 1536: 11.4 and 8.7), with 128 (row, key head) units up to 2048 (32 rows x 4: 13.6 and
+// 15.7), with 256 up to 4096 (64 rows x 4: 24.7 and 32.0; rows of 1 .. 4096 tokens 23.0 and 24.5), with 512 up to 8192 (128 rows x 4, 8192 tokens: 103
+// and 118; 256 rows x 8, up to 8000: 219 whole, 225 cut at 4096, 231 at 2048).  Longer rows of few units: as many workgroups as run at once, two to a
+// CU (3 rows x 4 key heads, 131001 tokens: 36.8 us at 512 workgroups, 39.8 at 768, 36.9 at 1024, 42.4 at 384); of many: 1024, so that rows of
+// different lengths even out.
 void cut(int64_t R, int64_t kv_heads, int64_t head_groups, int64_t max_len, int* chunk, int* splits) {
     const int64_t units = R * kv_heads * head_groups, target = units < 128 ? 512 : 1024;
-    int64_t c = (max_len * units + target - 1) / target;
+    const int64_t whole = units < 128 ? 1024 : (units < 256 ? 2048 : (units < 512 ? 4096 : 8192));
+    int64_t c = max_len <= whole ? max_len : (max_len * units + target - 1) / target;
     c = (c + 255) / 256 * 256;
     c = c < 256 ? 256 : (c > 8192 ? 8192 : c);
     *chunk = (int)c;
