@@ -382,3 +382,20 @@ def test_default_calls_are_what_they_were(T):
     a = T.InferenceState(dict(args))
     b = T.InferenceState(dict(args, repetition_penalty=1.0, frequency_penalty=0.0, presence_penalty=0))
     assert [s.tolist() for s in a.inference()] == [s.tolist() for s in b.inference()] and a.loop.rules is None and b.loop.rules is None
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
+def test_fewer_rows_of_long_contexts(T, dtype):
+    """A batch whose long contexts stay whole with all rows and are cut over workgroups once few are left."""
+    from tst_amd import kernels as K
+    lm, vocab = make_lm(T, dtype, d=128, heads=4, layers=1, pe_max_len=1500)
+    lens = [1400, 3] + [20] * 30
+    prompts = ragged(203, lens, 8)
+    z = torch.randn((32, 128), generator=torch.Generator().manual_seed(6)).cuda() * 0.1
+    sess = lm.paged_session(z, prompts, 2)
+    rows = K.RowState(32, 2, torch.device('cuda', 0), False, 0)
+    rows.sent.copy_(torch.arange(32, dtype=torch.int32))
+    rows.tok.copy_(torch.stack([p[-1] for p in prompts]))
+    every = sess.step(rows, 32, 0)[:32, :203].clone()
+    for n in (5, 2, 1):
+        assert_logits(sess.step(rows, n, 0)[:n, :203], every[:n], dtype)

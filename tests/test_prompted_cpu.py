@@ -70,6 +70,32 @@ def test_attn_cache4_work_is_a_pure_size_rule():
         K.attn_cache4_work(1, 4, 3, 64, 1)
 
 
+def test_attn_cache4_work_covers_fewer_rows_and_tokens():
+    """What a call asks for (its refusal says so) never exceeds what the size rule gives for at least as many rows and tokens."""
+    import random
+    rng, f = random.Random(3), _lib._dll.tst_attn_cache4_work
+
+    def wanted(r, heads, kv, dh, n):
+        with pytest.raises(_lib.TstError, match='are needed|not finite') as e:        # the scale is looked at after the scratch
+            _lib.call('tst_attn_cache4_f32', cache(kv_heads=kv, dh=dh), 16, heads * dh, 16, 4, 3, None, 16, n, 16, heads * dh, r, heads, float('nan'), None, 0,
+                      None)
+        text = str(e.value)
+        return int(text.split('floats, ')[1].split()[0]) if 'are needed' in text else 0
+
+    cut = 0
+    for _ in range(3000):
+        kv, dh = rng.choice([1, 2, 3, 4, 8, 16]), rng.choice([32, 64, 128, 256])
+        heads = kv * rng.choice([1, 2, 4, 16, 17, 40])
+        R, n = int(2 ** rng.uniform(0, 11)), int(2 ** rng.uniform(0, 18))
+        most = f(R, heads, kv, dh, n)
+        for r in {1, min(2, R), R, max(1, R // 2), rng.randint(1, R), min(R, max(1, 128 // kv)), min(R, max(1, 255 // kv)), min(R, max(1, 511 // kv))}:
+            for m in {n, rng.randint(1, n), max(1, n // 2), min(n, 1025), min(n, 2049), min(n, 4097), min(n, 8193)}:
+                need = wanted(r, heads, kv, dh, m)
+                cut += need > 0
+                assert need <= most, (r, R, heads, kv, dh, m, n)
+    assert cut > 1000
+
+
 @pytest.mark.parametrize('ty', ['f32', 'bf16'])
 def test_adjust_logits_refusals(ty):
     R = _lib.TstLogitRules

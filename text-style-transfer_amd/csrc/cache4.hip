@@ -762,8 +762,10 @@ int attn_cache4(const tst_cache4* c, const T* q, int64_t ldq, const int32_t* tab
     TST_REQUIRE(ldq % unit == 0 && ldo % unit == 0 && ldq >= heads * d.dh && ldo >= heads * d.dh, TST_ERR_ARG,
                 "%s: leading dimensions must hold heads * dh and be multiples of %d", who, (int)unit);
     TST_REQUIRE(tst_aligned16(q) && tst_aligned16(out) && tst_aligned16(work), TST_ERR_ARG, "%s: q, out and work must be 16-byte aligned", who);
-    const int64_t need = tst_attn_cache4_work(R, heads, d.kv_heads, d.dh, max_len);
-    TST_REQUIRE(need >= 0 && (need == 0 || (work != nullptr && n_work >= need)), TST_ERR_ARG, "%s: work holds %lld floats, %lld are needed", who,
+    int chunk, splits;
+    cut(R, d.kv_heads, (heads / d.kv_heads + 15) / 16, max_len, &chunk, &splits);
+    const int64_t need = splits > 1 ? R * heads * splits * (d.dh + 2) : 0;
+    TST_REQUIRE(need == 0 || (work != nullptr && n_work >= need), TST_ERR_ARG, "%s: work holds %lld floats, %lld are needed", who,
                 (long long)n_work, (long long)need);
     TST_REQUIRE(scale - scale == 0.0f, TST_ERR_ARG, "%s: scale is not finite", who);
     if (R == 0) return TST_OK;
@@ -800,9 +802,12 @@ extern "C" int tst_cache4_read_bf16(const tst_cache4* c, const int32_t* slots, v
 
 extern "C" int64_t tst_attn_cache4_work(int64_t R, int64_t heads, int64_t kv_heads, int64_t dh, int64_t max_len) {
     if (R < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dh < 1 || max_len < 0 || !tst_dims_ok({R, heads, dh, max_len})) return -1;
-    int chunk, splits;
-    cut(R, kv_heads, (heads / kv_heads + 15) / 16, max_len, &chunk, &splits);
-    return splits > 1 ? R * heads * splits * (dh + 2) : 0;
+    if (max_len <= 1024) return 0;                   // whole rows, however few
+    // The most partial results of any r <= R rows: chunks of at least max_len * units / target tokens are at most target / units + 1 of a row,
+    // and chunks of 8192, where that is more, ceil(max_len / 8192).
+    const int64_t per_row = kv_heads * ((heads / kv_heads + 15) / 16), most = R * ((max_len + 8191) / 8192), even = (1024 + per_row - 1) / per_row + R;
+    const int64_t parts = R * ((max_len + 255) / 256), cut_parts = most > even ? most : even;
+    return (parts < cut_parts ? parts : cut_parts) * heads * (dh + 2);
 }
 extern "C" int tst_attn_cache4_f32(const tst_cache4* c, const float* q, int64_t ldq, const int32_t* table, int64_t width, int64_t n_seq,
                                    const int32_t* seq, const int32_t* lens, int64_t max_len, float* out, int64_t ldo, int64_t R,

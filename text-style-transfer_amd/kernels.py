@@ -696,7 +696,7 @@ def cache4_read(cache, slots, k, v, n_rows):
 
 
 def attn_cache4_work(n_rows, heads, kv_heads, head_size, max_len, device='cuda'):
-    """The scratch tensor ``attn_cache4`` wants for calls of these sizes, or None where it needs none.  Calls that may run at the same
+    """The scratch tensor ``attn_cache4`` wants for calls of up to ``n_rows`` rows and ``max_len`` tokens, or None where it needs none.  Calls that may run at the same
     time (streams, captured graphs) need one each."""
     n = _lib._dll.tst_attn_cache4_work(n_rows, heads, kv_heads, head_size, max_len)
     if n < 0:
