@@ -399,3 +399,19 @@ def test_fewer_rows_of_long_contexts(T, dtype):
     every = sess.step(rows, 32, 0)[:32, :203].clone()
     for n in (5, 2, 1):
         assert_logits(sess.step(rows, n, 0)[:n, :203], every[:n], dtype)
+
+
+def test_paged_session_refusals(T):
+    lm, vocab = make_lm(T, 'fp32', layers=1, pe_max_len=50)
+    z = torch.zeros((2, 128), device='cuda')
+    ok = ragged(203, [5, 7], 1)
+    for args, why in [((z[:0], [], 3), 'at least one prompt'), ((z, ok, 0), 'max_new'), ((z, ok[:1], 3), 'conditioning vectors'), ((z[:, :64], ok, 3), 'model_size'),
+                      ((z, [ok[0], ok[1][:0]], 3), 'at least 1'), ((z, [ok[0], ok[1].float()], 3), '1-D tensor'), ((z, [ok[0], ok[1].view(1, -1)], 3), '1-D tensor'),
+                      ((z, ragged(203, [5, 49], 1), 3), 'positions exceed'), ((z, ok, 3, 24), 'page')]:
+        with pytest.raises(ValueError, match=why):
+            lm.paged_session(*args)
+    with pytest.raises(IndexError):
+        lm.paged_session(z, [ok[0], torch.tensor([1, 203])], 3)
+    lm.paged_session(z, ragged(203, [5, 48], 1), 3)                              # 48 + 3 - 1 positions
+    with pytest.raises(ValueError, match='head size'):
+        make_lm(T, 'fp32', d=96, heads=2, layers=1)[0].paged_session(z[:, :96].contiguous(), ok, 3)

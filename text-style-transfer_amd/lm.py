@@ -348,11 +348,15 @@ class PagedLMSession:
     def __init__(self, lm, z, prompts, max_new, page=32):
         if max_new < 1:
             raise ValueError('max_new must be at least 1')
+        if page not in (16, 32, 64, 128):
+            raise ValueError('a page holds 16, 32, 64 or 128 tokens, not %r' % (page,))
         self.lm, self.V = lm, lm.V
         dh = lm.d // lm.heads
         if dh not in (32, 64, 128, 256):
             raise ValueError('a 4-bit cache needs a head size of 32, 64, 128 or 256, the model has %d' % dh)
         self.z, toks, lens = _prompt_inputs(lm, z, prompts, 1, max_new - 1)
+        if not lens:
+            raise ValueError('a session needs at least one prompt')
         W = lm.prepared()
         dev, d = lm.device, lm.d
         B = len(lens)
