@@ -117,6 +117,24 @@ class Grammar:
         return table, pack_mask(table >= 0), start.to(device)
 
 
+# The soft step's distribution is softmax((softmax(x) + G) / temperature): a token whose logit the rules set to -inf has probability 0 there
+# and keeps its noise G, and penalties and biases end up squeezed into probabilities below 1.
+RULES_AND_GUMBEL = 'rules on logits do not hold for the distributions of gumbel=True: they cannot be combined'
+
+
+def _penalties(n_sent, repetition_penalty, frequency_penalty, presence_penalty):
+    """(repetition, frequency, presence) per sentence on the host, or None where they change nothing."""
+    rep = _per_sentence(repetition_penalty, n_sent, 'repetition_penalty', 0.0)
+    freq = _per_sentence(frequency_penalty, n_sent, 'frequency_penalty')
+    pres = _per_sentence(presence_penalty, n_sent, 'presence_penalty')
+    return (rep, freq, pres) if bool((rep != 1).any()) or bool((freq != 0).any()) or bool((pres != 0).any()) else None
+
+
+def any_rule(n_sent, repetition_penalty=1.0, frequency_penalty=0.0, presence_penalty=0.0, **others):
+    """Whether rules (the arguments of ``LogitRules``) would change any logits."""
+    return any(o is not None for o in others.values()) or _penalties(n_sent, repetition_penalty, frequency_penalty, presence_penalty) is not None
+
+
 class LogitRules:
     """What a decode call does to the logits before it picks tokens: penalties for repeated tokens, biases, token masks, a grammar.
     ``prompts``: token ids of every sentence before the first step (they count for the repetition penalty only).  The state per row is the
@@ -128,12 +146,10 @@ class LogitRules:
         self.V = V
         self.params = self.prompt = self.prompt_cu = self.bias = self.mask = self.table = self.state = None
         self.bias_by_sent = self.mask_by_sent = False
-        rep = _per_sentence(repetition_penalty, n_sent, 'repetition_penalty', 0.0)
-        freq = _per_sentence(frequency_penalty, n_sent, 'frequency_penalty')
-        pres = _per_sentence(presence_penalty, n_sent, 'presence_penalty')
-        if bool((rep != 1).any()) or bool((freq != 0).any()) or bool((pres != 0).any()):
-            self.params = torch.stack((rep, freq, pres), 1).contiguous().to(device)
-            if prompts is not None and bool((rep != 1).any()):
+        penalties = _penalties(n_sent, repetition_penalty, frequency_penalty, presence_penalty)
+        if penalties is not None:
+            self.params = torch.stack(penalties, 1).contiguous().to(device)
+            if prompts is not None and bool((penalties[0] != 1).any()):
                 lens = torch.tensor([0] + [len(p) for p in prompts], dtype=torch.int64)
                 self.prompt_cu = lens.cumsum(0).to(torch.int32).to(device)
                 self.prompt = torch.cat([torch.as_tensor(p).reshape(-1).to(device=device, dtype=torch.int32) for p in prompts])
@@ -209,6 +225,8 @@ class DecodeLoop:
         self.Ttot = self.pos0 + max_len
         if gumbel is not None and prefix is not None:
             raise ValueError('an id prefix and gumbel decoding cannot be combined')
+        if gumbel is not None and rules is not None and rules.active:
+            raise NotImplementedError(RULES_AND_GUMBEL)
         self.cur = K.RowState(R, self.Ttot, dev, session.needs_anc, pad)
         self.nxt = K.RowState(R, self.Ttot, dev, session.needs_anc, pad)
         self.sel = K.Selection(R, dev)

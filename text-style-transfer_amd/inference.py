@@ -24,7 +24,8 @@ B prompts (1-D id tensors) of different lengths.  Rounding keys and values to 4 
 ``frequency_penalty`` (times a token's count in the output, subtracted), ``presence_penalty`` (subtracted once) — each a number or one
 per sentence —, ``logit_bias`` (dict {id: bias}, or a tensor [V] or [B, V]), ``allowed_tokens`` (boolean [V] or [B, V]) and ``grammar``
 (an ``engine.Grammar``): rules applied to the logits of every step, in this order, before the token selection.  They work with every
-model, with beams (a hypothesis follows its own history and grammar state) and with sampling.
+model, with beams (a hypothesis follows its own history and grammar state) and with sampling; not with ``gumbel=True``, whose
+distributions would not keep them (``NotImplementedError``).
 
 ``active_seqs`` (``:37``): a caller-provided prefix of token ids ``[B, t0]`` replaces the single BOS; results start with
 it and may grow to ``t0 + max_len`` tokens (the loop still runs ``max_len`` steps, ``:155``).
@@ -43,7 +44,7 @@ per step exactly as the reference does, on GPU tensors, and only the selection /
 """
 import torch
 
-from .engine import DecodeLoop, LogitRules
+from .engine import RULES_AND_GUMBEL, DecodeLoop, LogitRules, any_rule
 
 
 class ForeignSession:
@@ -203,6 +204,8 @@ class InferenceState:
                     raise NotImplementedError("kv_cache='fp4' is supported for TransformerLM")
                 if self.beam_size != 1 or self.gumbel:
                     raise NotImplementedError("kv_cache='fp4' decodes one token sequence per sentence: no beams, no gumbel")
+            if self.gumbel and any_rule(self.batch_size, **self.rules):
+                raise NotImplementedError(RULES_AND_GUMBEL)
             if isinstance(self.active_seqs, (list, tuple)):
                 if self.kv_cache is None:
                     raise NotImplementedError("prompts of different lengths (active_seqs as a list) need kv_cache='fp4'")
