@@ -135,14 +135,52 @@ def any_rule(n_sent, repetition_penalty=1.0, frequency_penalty=0.0, presence_pen
     return any(o is not None for o in others.values()) or _penalties(n_sent, repetition_penalty, frequency_penalty, presence_penalty) is not None
 
 
+def _reached(next, is_open, starts, eos):
+    """Boolean [states]: what tokens of ``is_open`` [V] lead to from ``starts``; decoding ends with ``eos``."""
+    cols = is_open.nonzero().flatten()
+    cols = cols if eos is None else cols[cols != eos]
+    seen = torch.zeros(next.shape[0], dtype=torch.bool, device=next.device)
+    front = starts.long().unique()
+    while front.numel():
+        seen[front] = True
+        to = next[front][:, cols].flatten()
+        to = to[to >= 0].long().unique()
+        front = to[~seen[to]]
+    return seen
+
+
+def _check_tokens_left(bias, allowed, grammar, start, eos):
+    """Raises if ``bias`` [1 or n, V] forbids every token that ``allowed`` [1 or n, V] or a state of the grammar leaves a sentence: the
+    selection has no answer for a row of -inf.  A bias that rounds to -inf in bf16, the narrowest type of logits, forbids like -inf."""
+    is_open = torch.isfinite(bias.to(torch.bfloat16))
+    if bool(is_open.all()):
+        return
+    if grammar is None:
+        left = is_open if allowed is None else is_open & allowed
+        if not bool(left.any(1).all()):
+            raise ValueError('logit_bias leaves a sentence no token%s' % ('' if allowed is None else ' that allowed_tokens allows'))
+        return
+    next = grammar.next.to(bias.device)
+    empty = ((next >= 0).float() @ is_open.float().t() == 0).t()         # [1 or n, states]
+    met = {}
+    for b in empty.any(1).nonzero().flatten().tolist():
+        starts = start if is_open.shape[0] == 1 else start[b:b + 1]
+        key = None if is_open.shape[0] == 1 else (int(starts), is_open[b].cpu().numpy().tobytes())
+        if key not in met:
+            met[key] = _reached(next, is_open[b], starts, eos)
+        dead = (met[key] & empty[b]).nonzero().flatten()
+        if dead.numel():
+            raise ValueError('logit_bias leaves state %d of the grammar no token' % int(dead[0]))
+
+
 class LogitRules:
     """What a decode call does to the logits before it picks tokens: penalties for repeated tokens, biases, token masks, a grammar.
     ``prompts``: token ids of every sentence before the first step (they count for the repetition penalty only).  The state per row is the
     loop's own token history, and the grammar state of each row, which ``advance`` carries through selection, retirement and beam
-    reorders."""
+    reorders.  Rules that together leave a sentence no token are refused (``eos``: the token behind which nothing is picked)."""
 
     def __init__(self, V, n_sent, beam, device, repetition_penalty=1.0, frequency_penalty=0.0, presence_penalty=0.0, logit_bias=None,
-                 allowed_tokens=None, grammar=None, prompts=None):
+                 allowed_tokens=None, grammar=None, prompts=None, eos=None):
         self.V = V
         self.params = self.prompt = self.prompt_cu = self.bias = self.mask = self.table = self.state = None
         self.bias_by_sent = self.mask_by_sent = False
@@ -168,6 +206,7 @@ class LogitRules:
             self.bias = b.reshape(-1, V).to(device=device, dtype=torch.float32).contiguous()
         if allowed_tokens is not None and grammar is not None:
             raise ValueError('a grammar says which tokens are allowed: allowed_tokens cannot be given as well')
+        ok = start = None
         if allowed_tokens is not None:
             ok = torch.as_tensor(allowed_tokens)
             if tuple(ok.shape) not in ((V,), (n_sent, V)) or ok.dtype != torch.bool:
@@ -175,12 +214,15 @@ class LogitRules:
             if not bool(ok.reshape(-1, V).any(1).all()):
                 raise ValueError('allowed_tokens leaves a sentence no token')
             self.mask_by_sent = ok.dim() == 2
-            self.mask = pack_mask(ok.reshape(-1, V).to(device))
+            ok = ok.reshape(-1, V).to(device)
+            self.mask = pack_mask(ok)
         if grammar is not None:
             self.table, self.mask, start = grammar.on(device, n_sent, V)
             rows = n_sent * beam
             self.state, self.spare = (torch.full((rows,), -1, dtype=torch.int32, device=device) for _ in range(2))
             self.state[:n_sent] = start
+        if self.bias is not None:
+            _check_tokens_left(self.bias, ok, grammar, start, eos)
 
     @property
     def active(self):

@@ -25,7 +25,7 @@ B prompts (1-D id tensors) of different lengths.  Rounding keys and values to 4 
 per sentence —, ``logit_bias`` (dict {id: bias}, or a tensor [V] or [B, V]), ``allowed_tokens`` (boolean [V] or [B, V]) and ``grammar``
 (an ``engine.Grammar``): rules applied to the logits of every step, in this order, before the token selection.  They work with every
 model, with beams (a hypothesis follows its own history and grammar state) and with sampling; not with ``gumbel=True``, whose
-distributions would not keep them (``NotImplementedError``).
+distributions would not keep them (``NotImplementedError``), and not where they leave a sentence no token (``ValueError``).
 
 ``active_seqs`` (``:37``): a caller-provided prefix of token ids ``[B, t0]`` replaces the single BOS; results start with
 it and may grow to ``t0 + max_len`` tokens (the loop still runs ``max_len`` steps, ``:155``).
@@ -247,7 +247,8 @@ class InferenceState:
             with torch.cuda.device(device):
                 rules = None
                 if self.rules:
-                    rules = LogitRules(len(self.vocab), self.batch_size, self.beam_size, device, prompts=self._prompts(prefix), **self.rules)
+                    rules = LogitRules(len(self.vocab), self.batch_size, self.beam_size, device, prompts=self._prompts(prefix),
+                                       eos=self.eos_idx, **self.rules)
                 self.prompts = None
                 if self.kv_cache is not None:
                     # the session runs the prompts; the loop starts from their last tokens
