@@ -101,3 +101,12 @@ def test_biases_that_leave_a_state_of_the_grammar_nothing_are_refused():
         assert engine.LogitRules(V, 2, 1, 'cpu', logit_bias=b, grammar=engine.Grammar(chain(), start), eos=3).active
     with pytest.raises(ValueError, match='of the grammar no token'):     # without an end token 3 is a token like any other
         engine.LogitRules(V, 2, 1, 'cpu', logit_bias=bias_of([6]), grammar=engine.Grammar(chain(), 3))
+
+
+def test_a_forbidden_token_leaves_the_grammar_state_where_it_is():
+    """Beams and models with logits of -inf can pick a token that the state forbids: the row goes on under that state's rules, not under none."""
+    table, mask, start = engine.Grammar(chain(), [0, 2]).on('cpu', 2, V)
+    assert table.dtype == torch.int32 and table.is_contiguous()
+    want = torch.where(chain() < 0, torch.arange(4).unsqueeze(1), chain())
+    assert torch.equal(table.long(), want) and start.tolist() == [0, 2]
+    assert torch.equal(mask, engine.pack_mask(chain() >= 0))

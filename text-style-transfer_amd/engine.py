@@ -93,7 +93,8 @@ def pack_mask(allowed):
 
 class Grammar:
     """A finite automaton over tokens: ``next[s, v]`` (int [states, V]) is the state after token v in state s, -1 where v is
-    forbidden; decoding starts in state ``start`` (a number, or one per sentence).  Every state must allow some token."""
+    forbidden; decoding starts in state ``start`` (a number, or one per sentence).  Every state must allow some token.  A forbidden
+    token that comes up all the same (the model's own logits are -inf for all allowed ones) leaves the state as it is."""
 
     def __init__(self, next, start=0):
         t = torch.as_tensor(next)
@@ -113,8 +114,11 @@ class Grammar:
         start = start.expand(n_sent) if start.dim() == 0 else start
         if tuple(start.shape) != (n_sent,) or int(start.min()) < 0 or int(start.max()) >= self.next.shape[0]:
             raise ValueError('start must be a state, or one per sentence')
-        table = self.next.to(device).contiguous()
-        return table, pack_mask(table >= 0), start.to(device)
+        next = self.next.to(device)
+        # A forbidden token leaves the state where it is.  It can come up: in a beam with fewer allowed tokens than hypotheses, or where the
+        # model's own logits are -inf; state -1 would mean no rule at all for the rest of the row.
+        table = torch.where(next < 0, torch.arange(next.shape[0], dtype=torch.int32, device=device).unsqueeze(1), next).contiguous()
+        return table, pack_mask(next >= 0), start.to(device)
 
 
 # The soft step's distribution is softmax((softmax(x) + G) / temperature): a token whose logit the rules set to -inf has probability 0 there
