@@ -110,3 +110,11 @@ def test_a_forbidden_token_leaves_the_grammar_state_where_it_is():
     want = torch.where(chain() < 0, torch.arange(4).unsqueeze(1), chain())
     assert torch.equal(table.long(), want) and start.tolist() == [0, 2]
     assert torch.equal(mask, engine.pack_mask(chain() >= 0))
+
+
+def test_rules_for_another_vocabulary_than_the_models_are_refused():
+    """Columns behind the rules' vocabulary would pass as they are, forbidden or not."""
+    for n in (V - 1, V + 3):
+        rules = engine.LogitRules(V, 2, 1, 'cpu', allowed_tokens=torch.arange(V) < 5)
+        with pytest.raises(ValueError, match='%d tokens, the model has %d' % (V, n)):
+            engine.DecodeLoop(_Session(n), 2, 1, 5, 2, 3, 0, device=torch.device('cpu'), rules=rules)

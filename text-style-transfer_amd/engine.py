@@ -273,6 +273,8 @@ class DecodeLoop:
             raise ValueError('an id prefix and gumbel decoding cannot be combined')
         if gumbel is not None and rules is not None and rules.active:
             raise NotImplementedError(RULES_AND_GUMBEL)
+        if rules is not None and rules.active and rules.V != session.V:
+            raise ValueError('the rules are for a vocabulary of %d tokens, the model has %d' % (rules.V, session.V))
         self.cur = K.RowState(R, self.Ttot, dev, session.needs_anc, pad)
         self.nxt = K.RowState(R, self.Ttot, dev, session.needs_anc, pad)
         self.sel = K.Selection(R, dev)
