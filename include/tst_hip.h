@@ -679,8 +679,9 @@ int tst_grammar_next(const int32_t* next, int64_t n_states, int64_t V, const int
 /* One decode step of a transformer decoder stack without cross-attention (tst_tfm_step_run's model) whose rows stand at positions of
  * their own and whose self-attention reads a 4-bit paged cache: tst_page_step, embedding (pe[pos[r]]), per layer LayerNorm, q|k|v into
  * qkv, tst_cache4_write, tst_attn_cache4, output projection + residual, feed-forward; final LayerNorm; vocabulary projection into
- * step->logits.  `step` is the plan of tst_tfm_step_run (its caches, n_pos, anc_ld, part and argmax_keys are not used; n_pos bounds the
- * positions).  Host structs. */
+ * step->logits.  `step` is the plan of tst_tfm_step_run (its caches, anc_ld, part and argmax_keys are not used; pe holds n_pos positions, z, if
+ * any, n_seq rows).  0 <= t < max_len <= n_pos.  A row whose position base + t would be max_len or more, or whose sequence is outside
+ * 0 .. n_seq - 1, stores nothing, attends to nothing and gets logits without a meaning.  Host structs. */
 typedef struct tst_paged_step {
     const tst_tfm_step* step;
     const tst_cache4* caches;    /* host array of step->n_layers */
@@ -689,7 +690,7 @@ typedef struct tst_paged_step {
     int32_t *slots, *pos, *lens; /* [rows] work */
     void* qkv;                   /* [rows][3 d] work, the activation type */
     float* work;                 int64_t n_work;  /* for tst_attn_cache4 */
-    int64_t max_len;             /* upper bound of base + t + 1 over all steps */
+    int64_t max_len;             /* upper bound of base + t + 1 over all steps, at most step->n_pos */
 } tst_paged_step;
 int tst_paged_step_run(const tst_paged_step* p, const int32_t* tok, const int32_t* sent, int64_t R, int64_t t, void* stream);
 

@@ -145,13 +145,13 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(PlanArgs a) {
 __global__ __launch_bounds__(256) void page_step_kernel(const int32_t* __restrict__ base, const int32_t* __restrict__ sent, int64_t t,
                                                         const int32_t* __restrict__ table, int64_t width, int64_t n_seq, int page_shift,
                                                         int32_t* __restrict__ slots, int32_t* __restrict__ pos, int32_t* __restrict__ lens,
-                                                        int64_t R) {
+                                                        int64_t R, int64_t limit) {
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (r >= R) return;
     const int64_t s = sent != nullptr ? sent[r] : r;
     int32_t slot = -1, ps = 0, len = 0;
-    if (s >= 0 && s < n_seq) {
-        const int64_t p = (int64_t)max(base[s], 0) + t;
+    const int64_t p = s >= 0 && s < n_seq ? (int64_t)max(base[s], 0) + t : limit;
+    if (p < limit) {
         ps = clip31(p);
         len = clip31(p + 1);
         const int64_t j = p >> page_shift;
@@ -199,14 +199,20 @@ extern "C" int tst_page_plan(const int32_t* lens, const int32_t* room, int64_t B
     return tst_after_launch("tst_page_plan");
 }
 
-extern "C" int tst_page_step(const int32_t* base, const int32_t* sent, int64_t t, const int32_t* table, int64_t width, int64_t n_seq,
-                             int64_t page, int32_t* slots, int32_t* pos, int32_t* lens, int64_t R, void* stream) {
+// the rows' positions are below `limit`; others are treated like rows of no sequence
+int tst_page_step_within(const int32_t* base, const int32_t* sent, int64_t t, const int32_t* table, int64_t width, int64_t n_seq, int64_t page,
+                         int32_t* slots, int32_t* pos, int32_t* lens, int64_t R, int64_t limit, void* stream) {
     TST_REQUIRE(tst_dims_ok({t, width, n_seq, R}), TST_ERR_UNSUPPORTED, "tst_page_step: a size exceeds 2^31 - 1");
     TST_REQUIRE(t >= 0 && width >= 0 && n_seq >= 0 && R >= 0, TST_ERR_ARG, "tst_page_step: negative size");
     const int shift = page_shift_of(page);
     TST_REQUIRE(shift >= 0, TST_ERR_ARG, "tst_page_step: page must be a power of two in 8 .. 1024");
     TST_REQUIRE(R == 0 || (slots && pos && lens && (n_seq == 0 || (base && (width == 0 || table)))), TST_ERR_ARG, "tst_page_step: null pointer");
     if (R == 0) return TST_OK;
-    page_step_kernel<<<(unsigned)((R + 255) / 256), 256, 0, (hipStream_t)stream>>>(base, sent, t, table, width, n_seq, shift, slots, pos, lens, R);
+    page_step_kernel<<<(unsigned)((R + 255) / 256), 256, 0, (hipStream_t)stream>>>(base, sent, t, table, width, n_seq, shift, slots, pos, lens, R, limit);
     return tst_after_launch("tst_page_step");
+}
+
+extern "C" int tst_page_step(const int32_t* base, const int32_t* sent, int64_t t, const int32_t* table, int64_t width, int64_t n_seq,
+                             int64_t page, int32_t* slots, int32_t* pos, int32_t* lens, int64_t R, void* stream) {
+    return tst_page_step_within(base, sent, t, table, width, n_seq, page, slots, pos, lens, R, INT64_MAX, stream);
 }

@@ -354,7 +354,8 @@ extern "C" int tst_paged_step_run(const tst_paged_step* p, const int32_t* tok, c
     TST_REQUIRE(m->n_layers >= 1 && m->d > 0 && m->heads > 0 && m->d % m->heads == 0 && m->d_ff > 0 && m->V > 0, TST_ERR_ARG,
                 "tst_paged_step_run: bad sizes");
     TST_REQUIRE(R >= 0 && R <= m->slab_rows, TST_ERR_ARG, "tst_paged_step_run: %lld rows, buffers hold %lld", (long long)R, (long long)m->slab_rows);
-    TST_REQUIRE(t >= 0 && p->max_len >= 1 && p->max_len <= m->n_pos, TST_ERR_ARG, "tst_paged_step_run: max_len outside 1 .. n_pos");
+    TST_REQUIRE(t >= 0 && p->n_seq >= 0 && p->max_len >= 1 && p->max_len <= m->n_pos, TST_ERR_ARG, "tst_paged_step_run: max_len outside 1 .. n_pos");
+    TST_REQUIRE(t < p->max_len, TST_ERR_ARG, "tst_paged_step_run: step %lld outside 0 .. max_len - 1 = %lld", (long long)t, (long long)p->max_len - 1);
     TST_REQUIRE(m->x && m->h && m->a && m->ff && m->logits && p->slots && p->pos && p->lens && p->qkv, TST_ERR_ARG, "tst_paged_step_run: null work buffer");
     TST_REQUIRE(tok && m->emb && m->pe && m->wout && p->base && p->table, TST_ERR_ARG, "tst_paged_step_run: null input");
     TST_REQUIRE(m->z == nullptr || sent != nullptr, TST_ERR_ARG, "tst_paged_step_run: z without sent");
@@ -367,9 +368,9 @@ extern "C" int tst_paged_step_run(const tst_paged_step* p, const int32_t* tok, c
     if (R == 0) return TST_OK;
     const int64_t d = m->d, esz = m->bf16 != 0 ? 2 : 4;
     const StepCtx c{m, R, stream, m->bf16 != 0};
-    TST_TRY(tst_page_step(p->base, sent, t, p->table, p->width, p->n_seq, p->caches[0].page, p->slots, p->pos, p->lens, R, stream));
-    if (m->z != nullptr) TST_TRY(tst_embed_posadd_rows_f32(tok, m->emb, m->pe, p->pos, m->scale, m->z, sent, m->x, R, d, m->V, stream));
-    else TST_TRY(tst_embed_posadd_f32(tok, m->emb, m->pe, p->pos, m->scale, m->x, R, d, m->V, stream));
+    // base is on the device: positions are held below max_len, and so inside pe, there
+    TST_TRY(tst_page_step_within(p->base, sent, t, p->table, p->width, p->n_seq, p->caches[0].page, p->slots, p->pos, p->lens, R, p->max_len, stream));
+    TST_TRY(tst_embed_posadd_within_f32(tok, m->emb, m->pe, p->pos, m->scale, m->z, sent, p->n_seq, m->x, R, d, m->V, stream));
     const float scale = (float)(1.0 / sqrt((double)(d / m->heads)));
     char* qkv = (char*)p->qkv;
     for (int li = 0; li < m->n_layers; ++li) {

@@ -25,6 +25,12 @@ int tst_greedy_retire_compact_bounded(const int32_t* argmax_tok, const tst_rows*
 // rowops.hip: tst_embed_posadd_f32 / tst_embed_posadd_rows_f32 (z may be NULL) that also clears clear_keys[0..R) (arg-max keys)
 int tst_embed_posadd_clear_f32(const int32_t* tok, const float* emb, const float* pe, float scale, const float* z, const int32_t* zidx,
                                float* x, uint64_t* clear_keys, int64_t R, int64_t d, int64_t V, void* stream);
+// tst_embed_posadd_rows_f32 for rows that may belong to no sentence: where zidx is outside 0 .. n_z - 1 nothing is added (z may be NULL)
+int tst_embed_posadd_within_f32(const int32_t* tok, const float* emb, const float* pe, const int32_t* pos, float scale, const float* z,
+                                const int32_t* zidx, int64_t n_z, float* x, int64_t R, int64_t d, int64_t V, void* stream);
+// paged.hip: tst_page_step whose rows at positions from `limit` on are treated like rows of no sequence
+int tst_page_step_within(const int32_t* base, const int32_t* sent, int64_t t, const int32_t* table, int64_t width, int64_t n_seq, int64_t page,
+                         int32_t* slots, int32_t* pos, int32_t* lens, int64_t R, int64_t limit, void* stream);
 
 // gemm_f32_wreg.hip: the K = 256 product with the weights held in registers (used by tst_gemm_mfma_f32)
 bool tst_gemm_wreg_ok(int64_t M, int64_t N, int64_t K);

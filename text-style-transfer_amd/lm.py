@@ -360,7 +360,7 @@ class PagedLMSession:
         W = lm.prepared()
         dev, d = lm.device, lm.d
         B = len(lens)
-        self.R, self.page = B, page
+        self.R, self.page, self.max_new = B, page, max_new
         self.max_len = max(lens) + max_new - 1
         i32 = dict(dtype=torch.int32, device=dev)
         act = dict(dtype=torch.bfloat16 if lm.dtype == 'bf16' else torch.float32, device=dev)
@@ -395,6 +395,8 @@ class PagedLMSession:
         pass  # a row finds its pages through its sentence; nothing moves
 
     def step(self, rows, n, t):
-        """Logits of the next token of rows 0..n-1 (``rows.sent``, ``rows.tok``), each at position base + t of its sentence."""
+        """Logits of the next token of rows 0..n-1 (``rows.sent``, ``rows.tok``), each at position base + t of its sentence, t < max_new."""
+        if not 0 <= t < self.max_new:
+            raise ValueError('step %d of a session made for %d new tokens' % (t, self.max_new))
         self.plan.run(rows, n, t)
         return self.logits
