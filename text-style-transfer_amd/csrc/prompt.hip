@@ -10,7 +10,7 @@
 // The softmax needs a reference point per query, not the maximum: exp(s - r) sums and divides the same for every r that neither overflows
 // nor underflows it.  r is the largest score of the row's first tile; the score accumulators START at -r, so no subtraction, maximum or
 // rescaling of O is left in the loop (one exp2, one product and one sum per weight).  r moves when a sum has outgrown it by 2^60, and
-// rows whose result is not finite (one tile outgrew it by 2^127, a weight of 0 met an infinity) are computed again, plainly.
+// rows whose result is not finite (64 keys outgrew it by 2^127, a weight of 0 met an infinity) are computed again, plainly.
 //
 // What bounds it (dh 128, bf16): 64 keys x 32 queries cost a SIMD 1024 cycles of matrix instructions, and the four SIMDs together 1024
 // cycles of LDS reads (128 bytes per cycle), so both run full at the limit.  Two prompts of up to 8191 tokens, 16 heads over 4 key heads:
@@ -462,9 +462,10 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
         if (k0 == 0 || k0 + KT - 1 > qw) tile(std::true_type{});
         else tile(std::false_type{});
         if (DMA && !DOUBLE && k0 + KT <= q_end) fetch(k0 + KT, 0);            // the wave has used all it read
-        // The reference point moves when a sum has outgrown it by 2^60: far from any limit of fp32, and rare.  (A single tile that outgrows it by
-        // 2^127 overflows; its rows are computed again at the end.)
-        if (__ballot(sum > 0x1p60f) != 0ull) {
+        // The reference point moves when a sum has outgrown it by 2^60: far from any limit of fp32, and rare.  (64 keys that outgrow it by 2^127
+        // overflow; their rows are computed again at the end.)  It moves after every 64 keys and after the wave's last ones, whatever a tile
+        // holds: the same bits from every form of this kernel.
+        if ((KT % 64 == 0 || ((k0 + KT) & 63) == 0 || k0 + KT > w_end) && __ballot(sum > 0x1p60f) != 0ull) {
             const int by = __builtin_amdgcn_frexp_expf(fmaxf(fmaxf(sum, lane_xor<32>(sum)), 1.0f));     // (a factor 2^-by could be subnormal)
             const float raw = (float)by / a.scale2;
             sum = __builtin_amdgcn_ldexpf(sum, -by);
@@ -535,7 +536,7 @@ int launch_prompt(const PromptArgs& a, hipStream_t st, const char* who) {
     if constexpr (sizeof(T) == 2) {
         // Prompts of a few rows: one wave per workgroup, one tile of 32 keys in LDS, so that many are at work (256 prompts, 32 heads over 8 of
         // 128: 2 tokens each 19 us, 62 with four waves; 32 tokens 32 and 74; 64 tokens 86 and 110; 96 tokens 135 and 150, but of 8 heads of 64
-        // 27 and 22).  A row's sums run over the same keys in the same order either way.
+        // 27 and 22).  A row's sums run over the same keys in the same order, and its reference point moves at the same keys, either way.
         if (a.N / a.B <= 64) {
             if (a.dh == 32) return launch_one<T, 32, 32, true, 1>(a, st, who);
             if (a.dh == 64) return launch_one<T, 64, 32, true, 1>(a, st, who);
