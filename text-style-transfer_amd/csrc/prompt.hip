@@ -92,7 +92,7 @@ struct PromptArgs {
 // wait for it, not knowing that those read the other buffer; it writes no register, and the kernel waits for it before the barrier that
 // opens its buffer.
 __device__ __forceinline__ void dma16(uint32_t lds, const void* base, uint32_t offset) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds), "v"(offset), "s"(base) : "memory");
 }
 
 // LDS tiles are rows of DH / 8 chunks of 16 bytes.  Chunk c of row r sits at place c ^ swizzle(r), so that what an LDS read fetches in one
@@ -461,7 +461,10 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
         };
         if (k0 == 0 || k0 + KT - 1 > qw) tile(std::true_type{});
         else tile(std::false_type{});
-        if (DMA && !DOUBLE && k0 + KT <= q_end) fetch(k0 + KT, 0);            // the wave has used all it read
+        if (DMA && !DOUBLE && k0 + KT <= q_end) {                        // one buffer: the wave's reads of this tile are back before it is written
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            fetch(k0 + KT, 0);
+        }
         // The reference point moves when a sum has outgrown it by 2^60: far from any limit of fp32, and rare.  (64 keys that outgrow it by 2^127
         // overflow; their rows are computed again at the end.)  It moves after every 64 keys and after the wave's last ones, whatever a tile
         // holds: the same bits from every form of this kernel.
