@@ -630,7 +630,7 @@ int tst_cache4_read_bf16(const tst_cache4* c, const int32_t* slots, void* k, int
  *     out[r][h] = sum_p w_p V[p][g],   w = softmax_p(scale * q[r][h] . K[p][g]),   g = h / (heads / kv_heads)
  * A row with nothing to attend to (length 0 or less, a sequence outside 0 .. n_seq - 1) gives zeros; a page number outside the cache
  * counts as nothing to attend to.  q and out are fp32 or bf16 [R][ld >= heads * dh]; the keys and values enter the matrix cores as
- * they are (every code is exact in bf16); scores, softmax and sums are fp32.  heads % kv_heads == 0.
+ * they are (every code is exact in bf16); scores, softmax and sums are fp32, and weights keep 16 bits or more.  heads % kv_heads == 0.
  * max_len: an upper bound of lens known to the host.  work: scratch, written before it is read, not shared with a call that may run
  * at the same time; tst_attn_cache4_work gives the floats that suffice for calls of up to R rows and up to max_len tokens (0: NULL will
  * do), -1 for bad sizes. */

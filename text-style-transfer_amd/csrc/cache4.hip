@@ -247,11 +247,11 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Cache c, const int32_t
 //     after the four products: exactly the tokens whose value codes quarter j loads as 16 adjacent bytes.
 // Running maximum and sum are per lane (one head each); the maximum is shared by the four quarters through two lane exchanges, the sum
 // only at the end.  fp32 queries and weights enter as three bf16 pieces (8 + 8 + 8 bits of significand), the codes being exact: fp32
-// accuracy at three matrix instructions instead of one.  bf16 queries are one piece, and the weights are rounded to bf16 (half a step,
-// 2^-9 of a weight in [2^k, 2^(k+1)), against an output of 8 bits).
+// accuracy at three matrix instructions instead of one.  bf16 queries are one piece and their weights two: what is left of a weight in
+// [2^k, 2^(k+1)) is below 2^(k-16), so that the only rounding to bf16 is the output's.  (Weights of one piece, off by up to 2^(k-8): 218.5 us
+// instead of 221.5 for the 256 rows below, 36.7 instead of 37.7 for 3 rows of 131001 tokens, but 2.0e-3 instead of 1.7e-3 off the exact outputs.)
 //
-// Bound by memory: 256 rows of 8 key heads of 128, contexts of up to 8000 tokens (1.09 GB): 219 us, 5.0 TB/s, matrix instructions busy a
-// seventh of the time.  Long contexts are split over workgroups (rows x key heads x chunks) and, inside one, over its waves (tile by tile in turn); partial
+// Bound by memory: 256 rows of 8 key heads of 128, contexts of up to 8000 tokens (1.09 GB): 221 us, 4.9 TB/s.  Long contexts are split over workgroups (rows x key heads x chunks) and, inside one, over its waves (tile by tile in turn); partial
 // (maximum, sum, O) are joined in LDS and by combine_kernel, in a fixed order.
 
 union Frag {
@@ -366,7 +366,8 @@ __device__ __forceinline__ void load_values(ValueTile<DH>& t, const Cache& c, in
 
 template <typename T, int DH, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void attn_cache4_kernel(AttendArgs a) {
-    constexpr int NP = sizeof(T) == 4 ? 3 : 1;     // bf16 pieces of a query element or weight
+    constexpr int NP = sizeof(T) == 4 ? 3 : 1;     // bf16 pieces of a query element
+    constexpr int WP = sizeof(T) == 4 ? 3 : 2;     // and of a weight
     constexpr int KS = DH / 32;                    // steps of a key product
     constexpr int MT = DH / 16;                    // output tiles of 16 elements
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -480,7 +481,7 @@ __global__ __launch_bounds__(WAVES * 64) void attn_cache4_kernel(AttendArgs a) {
             m = top;
         }
         // the weights as the B operand: step st holds tokens 8 st .. 8 st + 7 of the quarter
-        uint32_t p[2][NP][4];
+        uint32_t p[2][WP][4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             float e[4];
@@ -489,11 +490,11 @@ __global__ __launch_bounds__(WAVES * 64) void attn_cache4_kernel(AttendArgs a) {
                 e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], a.scale2, -base));
                 sum += e[i];
             }
-            uint32_t x[NP], y[NP];
-            split2<NP>(e[0], e[1], x);
-            split2<NP>(e[2], e[3], y);
+            uint32_t x[WP], y[WP];
+            split2<WP>(e[0], e[1], x);
+            split2<WP>(e[2], e[3], y);
 #pragma unroll
-            for (int i = 0; i < NP; ++i) { p[u >> 1][i][2 * (u & 1)] = x[i]; p[u >> 1][i][2 * (u & 1) + 1] = y[i]; }
+            for (int i = 0; i < WP; ++i) { p[u >> 1][i][2 * (u & 1)] = x[i]; p[u >> 1][i][2 * (u & 1) + 1] = y[i]; }
         }
 #pragma unroll
         for (int b = 0; b < DH / 32; ++b) {
@@ -512,7 +513,7 @@ __global__ __launch_bounds__(WAVES * 64) void attn_cache4_kernel(AttendArgs a) {
 #pragma unroll
             for (int st = 0; st < 2; ++st)
 #pragma unroll
-                for (int i = 0; i < NP; ++i) {
+                for (int i = 0; i < WP; ++i) {
                     Frag pp;
                     pp.u[0] = p[st][i][0]; pp.u[1] = p[st][i][1]; pp.u[2] = p[st][i][2]; pp.u[3] = p[st][i][3];
                     o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even[st].v, pp.v, o[2 * b], 0, 0, 0);
