@@ -22,8 +22,13 @@
 // the diagonal.  In fp32, 16 prompts of 1 .. 60 tokens, 2 heads of 128: 10.0 us; 8 prompts of 2048, 8
 // heads of 64: 142 TFLOP/s, of 128: 129.  (With loads under a condition for heads smaller than the tile 12.6 us, 134 and 107.)
 //
-// fp32 inputs are split into three bf16 pieces (8 + 8 + 8 bits of significand, exactly the fp32 value) when a tile is staged, and the six
-// products of pieces down to 2^-18 of the largest are summed in fp32: what is left out is below 2^-26 of each product, and six bf16
+// bf16 rounds the weights to bf16 for the second product, off by up to 2^-8 of a weight, and the result once: 2.0e-3 .. 2.1e-3 off the exact
+// outputs in the two cases above, where fp32 weights leave 1.6e-3, the result's rounding alone.  It is a choice for speed: a second piece of the
+// weights makes it 1.6e-3, but half as many products again, and those are what bounds this kernel (491 -> 669 us, the ragged prompts 76 -> 84).
+//
+// fp32 inputs are split into three bf16 pieces (8 + 8 + 8 bits of significand, exactly the fp32 value; the second is at most 2^-8 of the
+// first's power of two, the third 2^-17) when a tile is staged, and the six products of pieces i and j with i + j <= 4 are summed in fp32: what
+// is left out is at most 2^-24 of each product (the largest found by enumeration 2^-24.04), half a step of fp32, and six bf16
 // instructions take 192 cycles where the fp32 matrix instructions would take 512.
 #include "tst_common.h"
 #include <type_traits>
