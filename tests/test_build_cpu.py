@@ -1,0 +1,32 @@
+"""CPU: what the build looks at: no kernel spills vector registers, and every source of the folder is one that is built."""
+import os
+import re
+import subprocess
+import sys
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'text-style-transfer_amd', 'csrc')
+
+REPORT = """unit.hip:10:1: remark: Function Name: kernel_a [-Rpass-analysis=kernel-resource-usage]
+   10 | __global__ void kernel_a() {
+unit.hip:10:1: remark:     VGPRs: 256 [-Rpass-analysis=kernel-resource-usage]
+unit.hip:10:1: remark:     ScratchSize [bytes/lane]: 0 [-Rpass-analysis=kernel-resource-usage]
+unit.hip:10:1: remark:     SGPRs Spill: 6 [-Rpass-analysis=kernel-resource-usage]
+unit.hip:10:1: remark:     VGPRs Spill: 0 [-Rpass-analysis=kernel-resource-usage]
+unit.hip:20:1: remark: Function Name: kernel_b [-Rpass-analysis=kernel-resource-usage]
+unit.hip:20:1: remark:     ScratchSize [bytes/lane]: 0 [-Rpass-analysis=kernel-resource-usage]
+unit.hip:20:1: remark:     VGPRs Spill: 0 [-Rpass-analysis=kernel-resource-usage]
+"""
+
+
+def check(report):
+    return subprocess.run([sys.executable, os.path.join(CSRC, 'check_spills.py'), 'unit'], input=report, capture_output=True, text=True)
+
+
+def test_a_kernel_that_spills_vector_registers_fails_the_build():
+    assert check(REPORT).returncode == 0 and check('').returncode == 0
+    head, tail = REPORT.rsplit('VGPRs Spill: 0', 1)
+    for bad in (head + 'VGPRs Spill: 12' + tail, REPORT.replace('lane]: 0', 'lane]: 48')):
+        r = check(bad)
+        assert r.returncode == 1 and 'kernel_b' in r.stderr
+    with open(os.path.join(CSRC, 'build.sh')) as f:
+        assert re.search(r'python3 check_spills.py \$1 < \S+ \|\| return 1', f.read())

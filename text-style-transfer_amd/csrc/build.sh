@@ -9,14 +9,21 @@ OUT=../libtst_hip.so
 # know the feature and says so: harmless).
 FLAGS="--offload-arch=gfx950 -O3 -fPIC -ffp-contract=off -std=c++17 -Wall -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
 UNITS="capi gemm_f32 gemm_f32_wreg gemm_f32_dma chain_f32 gemm_bf16 gru_fused rowops attn attn_mfma select gumbel paged cache4 prompt rules step"
+# One compile job; its kernels may not spill vector registers (check_spills.py says why).
+compile() {
+  /opt/rocm/bin/hipcc $FLAGS $2 -Rpass-analysis=kernel-resource-usage -c $1.hip -o $1.o.new 2> $1.o.log || { cat $1.o.log >&2; return 1; }
+  grep -A3 "warning:" $1.o.log >&2 || true
+  python3 check_spills.py $1 < $1.o.log || return 1
+  mv $1.o.new $1.o
+}
 pids=()
 for f in $UNITS; do
-  if [ ! -f $f.o ] || [ $f.hip -nt $f.o ] || [ build.sh -nt $f.o ] || [ tst_common.h -nt $f.o ] || [ ../../include/tst_hip.h -nt $f.o ]; then
+  if [ ! -f $f.o ] || [ $f.hip -nt $f.o ] || [ build.sh -nt $f.o ] || [ check_spills.py -nt $f.o ] || [ tst_common.h -nt $f.o ] || [ ../../include/tst_hip.h -nt $f.o ]; then
     rm -f $f.o
     EXTRA=""
     # the attention kernels do vector arithmetic on matrix accumulators all the time: keep those in ordinary registers
     case $f in cache4|prompt) EXTRA="-mllvm -amdgpu-mfma-vgpr-form=1" ;; esac
-    /opt/rocm/bin/hipcc $FLAGS $EXTRA -c $f.hip -o $f.o &
+    compile $f "$EXTRA" &
     pids+=($!)
   fi
 done
