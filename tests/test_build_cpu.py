@@ -30,3 +30,14 @@ def test_a_kernel_that_spills_vector_registers_fails_the_build():
         assert r.returncode == 1 and 'kernel_b' in r.stderr
     with open(os.path.join(CSRC, 'build.sh')) as f:
         assert re.search(r'python3 check_spills.py \$1 < \S+ \|\| return 1', f.read())
+
+
+def test_every_source_is_built():
+    """A kernel source that no build names is a stale copy of one that is."""
+    with open(os.path.join(CSRC, 'build.sh')) as f:
+        text = f.read()
+    units = re.search(r'^UNITS="([^"]+)"', text, re.M).group(1).split()
+    kept = subprocess.run(['git', 'ls-files', '--', '.'], cwd=CSRC, capture_output=True, text=True)
+    files = kept.stdout.split() if kept.returncode == 0 and kept.stdout else os.listdir(CSRC)
+    assert sorted(n[:-4] for n in files if n.endswith('.hip')) == sorted(units)
+    assert [n for n in files if n.endswith('.cpp')] == ['calls.cpp'] and 'calls.cpp' in text
