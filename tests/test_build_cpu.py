@@ -41,3 +41,16 @@ def test_every_source_is_built():
     files = kept.stdout.split() if kept.returncode == 0 and kept.stdout else os.listdir(CSRC)
     assert sorted(n[:-4] for n in files if n.endswith('.hip')) == sorted(units)
     assert [n for n in files if n.endswith('.cpp')] == ['calls.cpp'] and 'calls.cpp' in text
+
+
+def test_the_calls_module_is_for_this_torch():
+    import types
+
+    import pytest
+    import torch
+    from tst_amd import _lib
+    assert _lib.calls.built_for == torch.__version__.split('+')[0]
+    _lib._check_calls(_lib.calls)
+    for other in (types.SimpleNamespace(built_for='1.0.0'), types.SimpleNamespace()):
+        with pytest.raises(ImportError, match='build it with'):
+            _lib._check_calls(other)

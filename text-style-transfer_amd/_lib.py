@@ -200,9 +200,19 @@ class TstError(RuntimeError):
 _CALLS_PATH = os.path.join(_HERE, '_tst_calls.so')
 if not os.path.exists(_CALLS_PATH):
     raise ImportError('%s is missing: build it with text-style-transfer_amd/csrc/build.sh' % _CALLS_PATH)
+
+
+def _check_calls(module):
+    """The module reads torch's tensors in place: one that was built for another torch may not run."""
+    have, want = getattr(module, 'built_for', 'an unknown torch'), torch.__version__.split('+')[0]
+    if have != want:
+        raise ImportError('%s was built for torch %s, this is %s: build it with text-style-transfer_amd/csrc/build.sh' % (_CALLS_PATH, have, want))
+
+
 _spec = importlib.util.spec_from_file_location('_tst_calls', _CALLS_PATH)
 calls = importlib.util.module_from_spec(_spec)
 _spec.loader.exec_module(calls)
+_check_calls(calls)
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
 calls.bind({n: ctypes.cast(getattr(_dll, n), c_vp).value for n in _PROTOS}, getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device),
            _raw_stream if _raw_stream is not None else lambda dev: torch.cuda.current_stream(dev).cuda_stream, TstError)

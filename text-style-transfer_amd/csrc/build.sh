@@ -34,12 +34,15 @@ OBJS=""
 for f in $UNITS; do OBJS="$OBJS $f.o"; done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $OUT $OBJS
 # the checked calls of the prompted-decoding kernels, a host-only extension module
+# (its fields are torch's: another torch or Python wants another build)
 CALLS=../_tst_calls.so
-if [ ! -f $CALLS ] || [ calls.cpp -nt $CALLS ] || [ build.sh -nt $CALLS ] || [ ../../include/tst_hip.h -nt $CALLS ]; then
+FOR=$(python3 -c "import importlib.metadata as m, sys; print(m.version('torch'), sys.version)")
+if [ ! -f $CALLS ] || [ calls.cpp -nt $CALLS ] || [ build.sh -nt $CALLS ] || [ ../../include/tst_hip.h -nt $CALLS ] || [ "$(cat calls.o.for 2> /dev/null)" != "$FOR" ]; then
   rm -f $CALLS
   TORCH=$(python3 -c "import importlib.util as u; print(u.find_spec('torch').submodule_search_locations[0])")
   PY=$(python3 -c "import sysconfig; print(sysconfig.get_path('include'))")
   g++ -O2 -std=c++17 -fPIC -shared -fvisibility=hidden -Wall -D_GLIBCXX_USE_CXX11_ABI=1 -I../../include -I$PY -I$TORCH/include \
     -I$TORCH/include/torch/csrc/api/include calls.cpp -o $CALLS -L$TORCH/lib -ltorch_python -ltorch_cpu -lc10
+  echo "$FOR" > calls.o.for
 fi
 echo "built $OUT"

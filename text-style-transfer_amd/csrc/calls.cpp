@@ -9,6 +9,7 @@
 // entry point of libtst_hip.so whose address bind() was given (whichever build of the library the process loaded).
 #include "tst_hip.h"
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <cmath>
@@ -404,4 +405,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tst_calls", nullptr, -1, methods,
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit__tst_calls() { return PyModule_Create(&module); }
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__tst_calls() {
+    PyObject* m = PyModule_Create(&module);
+    // the tensor fields read here lie where this torch puts them: whoever loads the module compares
+    if (m != nullptr && PyModule_AddStringConstant(m, "built_for", TORCH_VERSION) != 0) Py_CLEAR(m);
+    return m;
+}
