@@ -631,7 +631,7 @@ int tst_cache4_read_bf16(const tst_cache4* c, const int32_t* slots, void* k, int
  * A row with nothing to attend to (length 0 or less, a sequence outside 0 .. n_seq - 1) gives zeros; a page number outside the cache
  * counts as nothing to attend to.  q and out are fp32 or bf16 [R][ld >= heads * dh]; the keys and values enter the matrix cores as
  * they are (every code is exact in bf16); scores, softmax and sums are fp32, and weights keep 16 bits or more.  heads % kv_heads == 0.
- * max_len: an upper bound of lens known to the host.  work: scratch, written before it is read, not shared with a call that may run
+ * max_len: an upper bound of lens known to the host, at most 2^31 - 1025.  work: scratch, written before it is read, not shared with a call that may run
  * at the same time; tst_attn_cache4_work gives the floats that suffice for calls of up to R rows and up to max_len tokens (0: NULL will
  * do), -1 for bad sizes. */
 int64_t tst_attn_cache4_work(int64_t R, int64_t heads, int64_t kv_heads, int64_t dh, int64_t max_len);

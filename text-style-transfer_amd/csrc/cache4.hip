@@ -659,6 +659,9 @@ __global__ __launch_bounds__(512) void attn_cache4_combine_kernel(AttendArgs a) 
     }
 }
 
+// Positions are counted in 32 bits, up to eight tiles ahead of the last token
+constexpr int64_t MOST_TOKENS = 0x7fffffff - 1024;
+
 // How a call is cut: tokens per workgroup (chunk) and how many chunks the longest row may have.  A second launch that joins chunks costs 3 us
 // and every chunk a prologue, so rows stay whole where walking one takes no longer: up to 1024 tokens (bf16, 4 key heads of 128, one row of
 // 512 tokens: 6.1 us whole, 8.6 cut; 1024 tokens: 8.0 and 8.7; 1536: 11.4 and 8.7), with 128 (row, key head) units up to 2048 (32 rows x 4: 13.6 and
@@ -757,6 +760,7 @@ int attn_cache4(const tst_cache4* c, const T* q, int64_t ldq, const int32_t* tab
     if (rc != TST_OK) return rc;
     TST_REQUIRE(tst_dims_ok({R, width, n_seq, max_len, heads}), TST_ERR_UNSUPPORTED, "%s: a size exceeds 2^31 - 1", who);
     TST_REQUIRE(R >= 0 && width >= 0 && n_seq >= 0 && max_len >= 0, TST_ERR_ARG, "%s: negative size", who);
+    TST_REQUIRE(max_len <= MOST_TOKENS, TST_ERR_UNSUPPORTED, "%s: max_len exceeds %lld", who, (long long)MOST_TOKENS);
     TST_REQUIRE(heads >= 1 && heads <= 4096 && heads % d.kv_heads == 0, TST_ERR_ARG, "%s: heads must be a multiple of kv_heads", who);
     TST_REQUIRE(R == 0 || (q && out && lens && (n_seq * width == 0 || table)), TST_ERR_ARG, "%s: null pointer", who);
     const int64_t unit = 16 / (int64_t)sizeof(T);
@@ -802,7 +806,7 @@ extern "C" int tst_cache4_read_bf16(const tst_cache4* c, const int32_t* slots, v
 }
 
 extern "C" int64_t tst_attn_cache4_work(int64_t R, int64_t heads, int64_t kv_heads, int64_t dh, int64_t max_len) {
-    if (R < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dh < 1 || max_len < 0 || !tst_dims_ok({R, heads, dh, max_len})) return -1;
+    if (R < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dh < 1 || max_len < 0 || max_len > MOST_TOKENS || !tst_dims_ok({R, heads, dh})) return -1;
     if (max_len <= 1024) return 0;                   // whole rows, however few
     // The most partial results of any r <= R rows: chunks of at least max_len * units / target tokens are at most target / units + 1 of a row,
     // and chunks of 8192, where that is more, ceil(max_len / 8192).
