@@ -665,7 +665,7 @@ typedef struct tst_logit_rules {
     const int32_t* mask_row;
 } tst_logit_rules;
 
-/* out[r][0..V) = the adjusted logits; out may be logits itself (same ld), else it must not overlap it. */
+/* out[r][0..V) = the adjusted logits; out may be logits itself (same ld), else it must not overlap it.  V <= 2^31 - 16385. */
 int tst_adjust_logits_f32(const float* logits, int64_t ld, int64_t R, int64_t V, const tst_logit_rules* rules, float* out,
                           int64_t ldo, void* stream);
 int tst_adjust_logits_bf16(const void* logits, int64_t ld, int64_t R, int64_t V, const tst_logit_rules* rules, void* out,

@@ -21,3 +21,14 @@ def test_attention_over_contexts_near_two_to_the_31(ty):
         assert _lib._dll.tst_attn_cache4_work(1, 4, 2, 64, n) == -1
     call(TOP - 1024)                        # no rows: nothing is launched
     assert _lib._dll.tst_attn_cache4_work(1, 4, 2, 64, TOP - 1024) > 0
+
+
+@pytest.mark.parametrize('ty', ['f32', 'bf16'])
+def test_rules_on_rows_near_two_to_the_31(ty):
+    """Columns are counted in chunks of up to 8192 from up to 7 in front of the row."""
+    def call(V):
+        _lib.call('tst_adjust_logits_' + ty, 16, TOP, 0, V, _lib.TstLogitRules(), 16, TOP, None)
+    for V in (TOP, TOP - 8191, TOP - 16383):
+        with pytest.raises(_lib.TstError, match='columns exceed'):
+            call(V)
+    call(TOP - 16384)

@@ -217,6 +217,8 @@ int adjust_logits(const T* logits, int64_t ld, int64_t R, int64_t V, const tst_l
     TST_REQUIRE(tst_dims_ok({R, V, a->n_sent, a->n_hist, a->n_prompt, a->n_bias, a->n_masks}), TST_ERR_UNSUPPORTED, "%s: a size exceeds 2^31 - 1", who);
     TST_REQUIRE(R >= 0 && V >= 0 && a->n_sent >= 0 && a->n_hist >= 0 && a->n_prompt >= 0 && a->n_bias >= 0 && a->n_masks >= 0, TST_ERR_ARG,
                 "%s: negative size", who);
+    constexpr int64_t MOST = 0x7fffffff - 2 * CHUNK_L;      // columns are counted in 32 bits, to the end of the last chunk
+    TST_REQUIRE(V <= MOST, TST_ERR_UNSUPPORTED, "%s: columns exceed %lld", who, (long long)MOST);
     TST_REQUIRE(R * V == 0 || (logits && out), TST_ERR_ARG, "%s: null pointer", who);
     TST_REQUIRE(ld >= V && ldo >= V, TST_ERR_ARG, "%s: leading dimensions must hold V columns", who);
     TST_REQUIRE((const void*)logits != (const void*)out || ld == ldo, TST_ERR_ARG, "%s: in place needs one leading dimension", who);
