@@ -32,3 +32,10 @@ def test_rules_on_rows_near_two_to_the_31(ty):
         with pytest.raises(_lib.TstError, match='columns exceed'):
             call(V)
     call(TOP - 16384)
+
+
+def test_scratch_of_calls_that_would_be_refused():
+    """rows * heads of a call fit 31 bits; beyond, the product of the scratch rule would not fit 64."""
+    f = _lib._dll.tst_attn_cache4_work
+    assert f(TOP, 4096, 1, 256, 1 << 30) == -1 and f(TOP, TOP, TOP, 256, 1 << 30) == -1 and f(1 << 20, 4096, 1, 256, 1 << 30) == -1
+    assert f((1 << 19) - 1, 4096, 1, 256, 1 << 30) > 0 and f(TOP, 1, 1, 32, 100) == 0 and f(TOP, 1, 1, 32, 1 << 30) > 0

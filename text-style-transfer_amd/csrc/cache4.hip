@@ -806,7 +806,7 @@ extern "C" int tst_cache4_read_bf16(const tst_cache4* c, const int32_t* slots, v
 }
 
 extern "C" int64_t tst_attn_cache4_work(int64_t R, int64_t heads, int64_t kv_heads, int64_t dh, int64_t max_len) {
-    if (R < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dh < 1 || max_len < 0 || max_len > MOST_TOKENS || !tst_dims_ok({R, heads, dh})) return -1;
+    if (R < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dh < 1 || max_len < 0 || max_len > MOST_TOKENS || !tst_dims_ok({R, heads, dh}) || !tst_dims_ok({R * heads})) return -1;
     if (max_len <= 1024) return 0;                   // whole rows, however few
     // The most partial results of any r <= R rows: chunks of at least max_len * units / target tokens are at most target / units + 1 of a row,
     // and chunks of 8192, where that is more, ceil(max_len / 8192).
