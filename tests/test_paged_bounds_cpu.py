@@ -41,3 +41,14 @@ def test_a_session_refuses_steps_behind_its_new_tokens():
             s.step(None, 1, t)
     s.step(None, 1, 2)
     assert s.plan.t == 2
+
+
+def test_a_paged_step_on_another_device_is_refused(monkeypatch):
+    """Like the wrappers: the kernels run on the current device, so the session has to live there."""
+    import torch
+    from tst_amd import kernels as K
+    plan = object.__new__(K.PagedPlan)
+    plan.dev = 1
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 0)
+    with pytest.raises(ValueError, match='the session is on cuda:1, the current device is cuda:0'):
+        plan.run(None, 1, 0)

@@ -733,6 +733,7 @@ class PagedPlan:
 
     def __init__(self, step, caches, table, base, rows, qkv, work, max_len):
         self._keep = [step, caches, table, base, qkv, work]
+        self.dev = table.get_device()
         i32 = dict(dtype=torch.int32, device=table.device)
         self.slots, self.pos, self.lens = _carve(torch.zeros(_arena_size([(rows,)] * 3), **i32), [(rows,)] * 3)
         self._caches = (_lib.TstCache4 * len(caches))(*[c.c for c in caches])
@@ -741,4 +742,7 @@ class PagedPlan:
                                    work=_p(work), n_work=0 if work is None else work.numel(), max_len=max_len)
 
     def run(self, rows, n_rows, t):
+        now = torch.cuda.current_device()
+        if now != self.dev:
+            raise ValueError('the session is on cuda:%d, the current device is cuda:%d' % (self.dev, now))
         call('tst_paged_step_run', self.c, _p(rows.tok), _p(rows.sent), n_rows, t, _stream())
