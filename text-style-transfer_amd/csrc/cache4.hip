@@ -664,10 +664,10 @@ constexpr int64_t MOST_TOKENS = 0x7fffffff - 1024;
 
 // How a call is cut: tokens per workgroup (chunk) and how many chunks the longest row may have.  A second launch that joins chunks costs 3 us
 // and every chunk a prologue, so rows stay whole where walking one takes no longer: up to 1024 tokens (bf16, 4 key heads of 128, one row of
-// 512 tokens: 6.1 us whole, 8.6 cut; 1024 tokens: 8.0 and 8.7; 1536: 11.4 and 8.7), with 128 (row, key head) units up to 2048 (32 rows x 4: 13.6 and
-// 15.7), with 256 up to 4096 (64 rows x 4: 24.7 and 32.0; rows of 1 .. 4096 tokens 23.0 and 24.5), with 512 up to 8192 (128 rows x 4, 8192 tokens: 103
-// and 118; 256 rows x 8, up to 8000: 219 whole, 225 cut at 4096, 231 at 2048).  Longer rows of few units: as many workgroups as run at once, two to a
-// CU (3 rows x 4 key heads, 131001 tokens: 36.8 us at 512 workgroups, 39.8 at 768, 36.9 at 1024, 42.4 at 384); of many: 1024, so that rows of
+// 512 tokens: 6.6 us whole, 8.8 cut; 1024 tokens: 8.7 and 8.7; 1536: 10.8 and 8.8), with 128 (row, key head) units up to 2048 (32 rows x 4: 14.3 and
+// 15.1), with 256 up to 4096 (64 rows x 4: 26.3 and 30.4; rows of 1 .. 4096 tokens 24.2 and 25.0), with 512 up to 8192 (128 rows x 4, 8192 tokens: 105
+// and 110; 256 rows x 8, up to 8000: 220 both).  Longer rows of few units: as many workgroups as run at once, two to a CU (3 rows x 4 key heads,
+// 131001 tokens: 37.7 us at 512 workgroups, 40.8 at 768, 37.5 at 1024 with twice the partial results, 44.5 at 384); of many: 1024, so that rows of
 // different lengths even out.
 void cut(int64_t R, int64_t kv_heads, int64_t head_groups, int64_t max_len, int* chunk, int* splits) {
     const int64_t units = R * kv_heads * head_groups, target = units < 128 ? 512 : 1024;

@@ -638,7 +638,8 @@ _calls = _lib.calls
 def attn_prompt(q, k, v, cu, out, heads, kv_heads=None, scale=None):
     """Causal attention over packed prompts: rows cu[b] .. cu[b + 1] - 1 of q [N, heads * dh], k, v [N, kv_heads * dh] (views with
     unit inner stride, fp32 or bf16) are sequence b; head h reads key head h // (heads / kv_heads).  ``out`` [N, heads * dh] must not
-    overlap them; its rows outside every sequence are left alone.  ``scale``: 1 / sqrt(dh) unless given."""
+    overlap them; its rows outside every sequence are left alone (let q end with the last sequence: rows per sequence choose the kernel's
+    form).  ``scale``: 1 / sqrt(dh) unless given."""
     _calls.attn_prompt(q, k, v, cu, out, heads, kv_heads, scale)
 
 
