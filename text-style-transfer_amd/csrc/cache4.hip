@@ -251,7 +251,8 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Cache c, const int32_t
 // [2^k, 2^(k+1)) is below 2^(k-16), so that the only rounding to bf16 is the output's.  (Weights of one piece, off by up to 2^(k-8): 218.5 us
 // instead of 221.5 for the 256 rows below, 36.7 instead of 37.7 for 3 rows of 131001 tokens, but 2.0e-3 instead of 1.7e-3 off the exact outputs.)
 //
-// Bound by memory: 256 rows of 8 key heads of 128, contexts of up to 8000 tokens (1.09 GB): 221 us, 4.9 TB/s.  Long contexts are split over workgroups (rows x key heads x chunks) and, inside one, over its waves (tile by tile in turn); partial
+// Bound by memory: 256 rows of 8 key heads of 128, contexts of up to 8000 tokens (1.09 GB): 221 us, 4.9 TB/s, matrix instructions busy a
+// quarter of the time.  Long contexts are split over workgroups (rows x key heads x chunks) and, inside one, over its waves (tile by tile in turn); partial
 // (maximum, sum, O) are joined in LDS and by combine_kernel, in a fixed order.
 
 union Frag {
