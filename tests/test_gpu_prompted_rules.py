@@ -54,3 +54,31 @@ def test_gumbel_with_neutral_rules_runs_and_with_rules_is_refused(T):
     assert all(torch.equal(x, y) for x, y in zip(a, b))
     with pytest.raises(NotImplementedError, match='gumbel'):
         T.InferenceState(dict(args, allowed_tokens=torch.arange(V) < 50)).inference()
+
+
+@pytest.mark.parametrize('beam', [1, 4])
+@pytest.mark.parametrize('kind', ['transformer', 'rnnlm', 'lm_fp32', 'lm_bf16', 'lm_4bit'])
+def test_rules_that_change_no_logit_change_no_result(T, kind, beam):
+    """With rules the selection reads the whole rows of logits instead of what a model's own projection left for it: the same results."""
+    from tst_amd import synthetic
+    if kind == 'lm_4bit' and beam > 1:
+        pytest.skip('the 4-bit cache decodes without beams')
+    vocab, B, extra = T.Vocab.synthetic(1203), 600, {}
+    g = torch.Generator().manual_seed(3)
+    if kind == 'transformer':
+        m = T.Transformer(T.HP(dict(d_model=64, dropout=0.1, n_layers=2, pe_max_len=60, n_heads=2, d_ff=128)), vocab, vocab)
+        model, x = m.decoder, torch.randn((B, 9, 64), generator=g).cuda()
+    elif kind == 'rnnlm':
+        m = model = T.RNNLM(64, vocab, 2)
+        x, extra = torch.randn((2, B, 64), generator=g).cuda(), {'substitute_inputs': True, 'inputs_batch_dim': 1, 'kwargs': {'return_z': True}}
+    else:
+        m = model = T.TransformerLM(T.HP(dict(model_size=128, n_layers=2, n_heads=2, d_ff=256, pe_max_len=60)), vocab,
+                                    dtype='fp32' if kind == 'lm_fp32' else 'bf16')
+        x, extra = torch.randn((B, 128), generator=g).cuda() * 0.1, {'kv_cache': 'fp4'} if kind == 'lm_4bit' else {}
+    m.load_state_dict(synthetic.synthetic_state_dict(m, 3, 1.0, 2.0, seed=4))
+    args = {'model': model, 'inputs': x, 'vocab': vocab, 'max_len': 10, 'beam_size': beam, **extra}
+    tok, n, _ = T.InferenceState(dict(args)).decode_packed()
+    for rule in (dict(logit_bias=torch.zeros(1203)), dict(allowed_tokens=torch.ones(B, 1203, dtype=torch.bool)),
+                 dict(grammar=T.Grammar(torch.zeros(1, 1203, dtype=torch.int64)))):
+        got = T.InferenceState(dict(args, **rule)).decode_packed()
+        assert torch.equal(got[0], tok) and torch.equal(got[1], n), list(rule)
