@@ -589,7 +589,7 @@ int tst_page_step(const int32_t* base, const int32_t* sent, int64_t t, const int
  * Replaces the self-attention of a model run on whole prefixes (/root/reference/src/inference.py:132).
  * heads % kv_heads == 0; dh <= 256, a multiple of 8 (bf16) or 4 (fp32); leading dimensions likewise (ldk, ldv <= 2^22), 16-byte
  * aligned pointers; a finite scale.
- * Scores, softmax and sums are fp32; the bf16 form rounds the weights to bf16 for the product with v, and the result once. */
+ * Scores, softmax and sums are fp32; the bf16 form rounds the weights to bf16, for the product with v and for their sum alike, and the result once. */
 int tst_attn_prompt_f32(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv, const int32_t* cu,
                         int64_t B, float* out, int64_t ldo, int64_t N, int64_t heads, int64_t kv_heads, int64_t dh, float scale,
                         void* stream);

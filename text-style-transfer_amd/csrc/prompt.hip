@@ -22,8 +22,10 @@
 // the diagonal.  In fp32, 16 prompts of 1 .. 60 tokens, 2 heads of 128: 10.0 us; 8 prompts of 2048, 8
 // heads of 64: 142 TFLOP/s, of 128: 129.  (With loads under a condition for heads smaller than the tile 12.6 us, 134 and 107.)
 //
-// bf16 rounds the weights to bf16 for the second product, off by up to 2^-8 of a weight, and the result once: 2.0e-3 .. 2.1e-3 off the exact
-// outputs in the two cases above, where fp32 weights leave 1.6e-3, the result's rounding alone.  It is a choice for speed: a second piece of the
+// bf16 rounds the weights to bf16 for the second product, off by up to 2^-8 of a weight, and sums the ROUNDED weights (v_dot2, two at a time; fp32
+// sums): what is common to a row's weights divides out, so a row that few keys take loses nothing (scores of 30 standard deviations, 8191
+// tokens: 1.26e-3 off the exact outputs, 1.99e-3 with the sum of the unrounded weights, 1.21e-3 the result's own rounding).  Rows that all keys
+// share remain: 2.0e-3 .. 2.1e-3 in the two cases above, where fp32 weights leave 1.6e-3.  That is a choice for speed: a second piece of the
 // weights makes it 1.6e-3, but half as many products again, and those are what bounds this kernel (491 -> 669 us, the ragged prompts 76 -> 84).
 //
 // fp32 inputs are split into three bf16 pieces (8 + 8 + 8 bits of significand, exactly the fp32 value; the second is at most 2^-8 of the
@@ -432,7 +434,7 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     sc[n][i] = __builtin_amdgcn_exp2f(sc[n][i] * a.scale2);
-                    sum += sc[n][i];
+                    if (NP == 3) sum += sc[n][i];
                 }
                 // step s of the second product: 16 keys, the half's 8 in registers 8 (s & 1) .. of the weights of 32-key block s / 2
 #pragma unroll
@@ -443,6 +445,8 @@ __global__ __launch_bounds__(64 * WAVES, DMA && DH <= 128 ? 2 : 1) void attn_pro
                         for (int i = 0; i < 4; ++i) {
                             const int at = 8 * (s & 1) + 2 * i;
                             p[s][x].u[i] = pack2(sc[n][at], sc[n][at + 1]);
+                            if (NP == 1)                              // the sum of the weights as they are multiplied
+                                sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p[s][x].u[i]), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
                             if (x + 1 < NP) {
                                 sc[n][at] -= low_f(p[s][x].u[i]);
                                 sc[n][at + 1] -= high_f(p[s][x].u[i]);
